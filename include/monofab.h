@@ -131,6 +131,71 @@ int monofab_attention(const void* q, const void* k_cache, const void* v_cache, v
                       int n_pages, float scale_log2, float* ws, int ws_rows, const int32_t* merge_items, int n_merge,
                       int32_t* status, void* stream);
 
+/* Paged-KV GQA attention with a window and a few first keys that stay visible, or with a tree of drafted tokens
+ * behind the past (the reference has neither; it stands beside its attention tiles,
+ * csrc/fabric/tiles/attention.cuh:174-395).  All lengths are read on the device, so a captured call may be replayed with
+ * others.  Request r's rows are rows q_start[r] .. q_start[r + 1] - 1 of q and out, the last of its kv_len[r] keys are
+ * those of its rows: row i is at position p = kv_len - rows + i.  The keys that it sees are
+ *   tree == NULL:  j <= p and (j > p - window or j < sinks);
+ *   else           the past (j < kv_len - rows) and the drafted tokens whose bit is set: of drafted token d bit d % 32 of
+ *                  tree[row][d / 32]; those from 32 * words on have none.
+ * out = sum_j softmax_j(scale q k_j) v_j; a row that sees no key is zeros.  Rows of no request keep what they hold.
+ * Values of keys that a request's row sees must be finite, also for that request's rows that do not see them; what no row
+ * of a request sees may hold anything.
+ * Keys past the block table (kv_len > bt_stride * page_size) are not there; a page number outside [0, n_pages) reads as
+ * zeros; q_start is taken as ascending within [0, tokens], and a request that it gives no rows has none. */
+typedef struct {
+  const void* q;               /* [tokens][hq][head_dim], rows q_row values apart, heads q_head; 16-bit values */
+  const void* k_cache;         /* [n_pages][page_size][hkv][head_dim] */
+  const void* v_cache;
+  void* out;                   /* [tokens][hq][head_dim], rows out_row values apart, heads out_head */
+  const int32_t* block_table;  /* [requests][bt_stride] */
+  const int32_t* q_start;      /* [requests + 1] */
+  const int32_t* kv_len;       /* [requests] */
+  const int32_t* tree;         /* [tokens][words], or NULL */
+  void* ws;                    /* monofab_masked_attention_ws_bytes(...) bytes that the call may overwrite; calls whose kernels
+                                  overlap on the GPU need one each */
+  int32_t* status;             /* receives MONOFAB_STATUS_WAIT_TIMEOUT if a bounded wait ran out; NULL: the device's own word */
+  int64_t q_row, q_head, out_row, out_head, ws_bytes;
+  int32_t tokens, requests, hq, hkv, head_dim, page_size, n_pages, bt_stride;
+  int32_t words, window, sinks;
+  int32_t fp16;                /* 0: bf16 values, else fp16 */
+  float scale;                 /* of the scores, positive */
+  int32_t reserved;
+} monofab_masked_attention_args;
+size_t monofab_masked_attention_ws_bytes(int tokens, int hq, int hkv, int head_dim);
+int monofab_masked_attention(const monofab_masked_attention_args* args, void* stream);
+/* The current device's own status word of these calls, read (the device is synchronised) and cleared. */
+int monofab_masked_attention_status(int32_t* out);
+
+/* Norms of queries and keys for each head, position rotation and append to the paged caches in one pass: the qk tile
+ * (csrc/fabric/tiles/aux.cuh:232-320) as a launch on a stream, with 32-bit arithmetic throughout and one rounding.
+ * qkv: T rows of hq q, hkv k and hkv v heads, ld_qkv values apart; q and k heads: x * rsqrt(mean(x^2) + eps) * norm weight
+ * (NULL: no norm), then the first rot dims turned by (cos, sin) = cos_sin[position], fp32 [max_pos][rot / 2][2]: pairs
+ * (d, d + rot / 2), or (2 d, 2 d + 1) if interleaved; positions outside the table take its nearest row.  q heads go to
+ * q_out (rows ld_out values apart; may be the q heads of qkv themselves), k and v heads to slot (page * page size + row in
+ * the page) slots[t] of caches [n_slots][hkv][head_dim]; slots outside [0, n_slots) (padding: -1) store nothing.  Rows
+ * stored in one slot in one call leave one or the other's values there.  head_dim 64, 128 or 256; values bf16, or fp16. */
+int monofab_qk_rope(const void* qkv, int64_t ld_qkv, const int32_t* positions, const int32_t* slots, const float* cos_sin,
+                    int max_pos, const void* q_norm, const void* k_norm, void* q_out, int64_t ld_out, void* k_cache,
+                    void* v_cache, int64_t n_slots, int T, int hq, int hkv, int head_dim, int rot, int interleaved, int fp16,
+                    float eps, void* stream);
+
+/* Page dst[i] takes what page src[i] holds, in all n_tensors cache tensors (device array of addresses, each
+ * [n_pages][page_bytes], 16-byte aligned).  A pair whose page numbers lie outside [0, n_pages), whose destination is
+ * another pair's source or destination or whose source is another's destination is not copied, and `status` (device
+ * int32) receives MONOFAB_STATUS_BAD_ARGS.  At most 65535 pairs and tensors. */
+int monofab_page_copy(const uint64_t* tensors, int n_tensors, const int32_t* src, const int32_t* dst, int pairs, int n_pages,
+                      int64_t page_bytes, int32_t* status, void* stream);
+
+/* Row base[r] + path[r][i] of request r moves to row base[r] + i, i < min(count[r], most), in all tensors
+ * ([n_pages][page_size][row_bytes]); every row is read before any is overwritten.  A row whose place lies outside the
+ * block table (int32 [requests][bt_stride]) or the pages is not moved, and `status` receives MONOFAB_STATUS_BAD_ARGS.
+ * Requests must not share the pages of these rows.  most <= 2048. */
+int monofab_accept_rows(const uint64_t* tensors, int n_tensors, const int32_t* block_table, int bt_stride,
+                        const int32_t* base, const int32_t* path, const int32_t* count, int requests, int most,
+                        int page_size, int n_pages, int64_t row_bytes, int32_t* status, void* stream);
+
 /* Diagnostics of the attention kernel (no counterpart in the reference): enable or
  * disable the phase trace of work item 0, and read the last one (out may be NULL):
  * cycles waiting for S, in the max pass, in exp + P store, rescaling O (tiles where a

@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("MONOFAB_LIB") or os.path.join(_HERE, "libmonofab.so")
 # Every symbol include/monofab.h declares; tests check that all of them resolve.
 EXPORTS = [
     "monofab_version", "monofab_last_error", "monofab_struct_layouts_json", "monofab_host_device_pointer",
-    "monofab_host_alloc", "monofab_host_free", "monofab_router_logits", "monofab_router_topk", "monofab_combine", "monofab_attention", "monofab_attention_trace", "monofab_pack_scratch_bytes", "monofab_pack_pairs", "monofab_pack_pairs_static",
+    "monofab_host_alloc", "monofab_host_free", "monofab_router_logits", "monofab_router_topk", "monofab_combine", "monofab_attention", "monofab_attention_trace", "monofab_masked_attention_ws_bytes", "monofab_masked_attention", "monofab_masked_attention_status", "monofab_qk_rope", "monofab_page_copy", "monofab_accept_rows", "monofab_pack_scratch_bytes", "monofab_pack_pairs", "monofab_pack_pairs_static",
     "monofab_moe_create", "monofab_moe_destroy", "monofab_moe_set_router", "monofab_moe_set_region",
     "monofab_moe_set_scales", "monofab_pack_w13", "monofab_moe_set_w13_packed", "monofab_moe_set_table", "monofab_moe_set_plan", "monofab_moe_forward", "monofab_moe_experts",
     "monofab_moe_forward_host", "monofab_moe_status", "monofab_moe_workspace", "monofab_moe_set_profile",
@@ -53,6 +53,15 @@ class MoEConfigC(ctypes.Structure):
                 ("reserved", ctypes.c_int32 * 7)]
 
 
+class MaskedAttentionArgsC(ctypes.Structure):
+    """struct monofab_masked_attention_args of include/monofab.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k_cache", "v_cache", "out", "block_table", "q_start", "kv_len", "tree", "ws", "status")] +
+                [(n, ctypes.c_int64) for n in ("q_row", "q_head", "out_row", "out_head", "ws_bytes")] +
+                [(n, ctypes.c_int32) for n in ("tokens", "requests", "hq", "hkv", "head_dim", "page_size", "n_pages", "bt_stride",
+                                               "words", "window", "sinks", "fp16")] +
+                [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing: build it with `python -m monoserve_b200.build` "
@@ -72,6 +81,14 @@ def _load():
     lib.monofab_pack_pairs_static.argtypes = [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.monofab_attention.argtypes = [vp, vp, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, i32, vp, i32, vp, vp]
     lib.monofab_attention_trace.argtypes = [i32, vp]
+    i64 = ctypes.c_int64
+    lib.monofab_masked_attention_ws_bytes.restype = ctypes.c_size_t
+    lib.monofab_masked_attention_ws_bytes.argtypes = [i32, i32, i32, i32]
+    lib.monofab_masked_attention.argtypes = [ctypes.POINTER(MaskedAttentionArgsC), vp]
+    lib.monofab_masked_attention_status.argtypes = [ctypes.POINTER(ctypes.c_int32)]
+    lib.monofab_qk_rope.argtypes = [vp, i64, vp, vp, vp, i32, vp, vp, vp, i64, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, f32, vp]
+    lib.monofab_page_copy.argtypes = [vp, i32, vp, vp, i32, i32, i64, vp, vp]
+    lib.monofab_accept_rows.argtypes = [vp, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i64, vp, vp]
     lib.monofab_combine.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, f32, vp]
     lib.monofab_moe_create.argtypes = [ctypes.POINTER(MoEConfigC), ctypes.POINTER(vp)]
     lib.monofab_moe_destroy.argtypes = [vp]
@@ -161,7 +178,6 @@ def _load():
     lib.monofab_plan_deadline_floor.argtypes = [vp, vp, f64, i32, P(i32)]
     lib.monofab_plan_solve.argtypes = [vp, vp, i32, u64, vp, i32]
     lib.monofab_plan_clear_cache.argtypes = [vp]
-    i64 = ctypes.c_int64
     lib.monofab_plan_profile_create.argtypes = [i32, i32, P(vp)]
     lib.monofab_plan_profile_destroy.argtypes = [vp]
     lib.monofab_plan_profile_set.argtypes = [vp, i32, vp, i32]

@@ -138,3 +138,108 @@ def fabric_tiles(items, merge, args_ptr, kind=K_ATTN_PREFILL):
     merges = tile_array(K_ATTN_MERGE, i0=mg[:, 0], i1=mg[:, 1] | (mg[:, 2] << 16), i2=mg[:, 3],
                         i3=mg[:, 4] | (mg[:, 5] << 16), a0=args_ptr)
     return tiles, merges
+
+
+# ------------------------------------------------------------------ windows and sinks, trees of drafted tokens
+
+_HALVES = (torch.bfloat16, torch.float16)
+
+
+def _refuse(ok, what):
+    if not ok:
+        raise ValueError("monofab: " + what)
+
+
+def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window, sinks, tree, scale, out, stream, status):
+    _refuse(q.dim() == 3 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape,
+            "q is [tokens, hq, head_dim], the caches are [pages, page_size, hkv, head_dim]")
+    T, hq, D = q.shape
+    n_pages, page, hkv, Dk = k_cache.shape
+    _refuse(D == Dk and D in (64, 128), f"head_dim must be 64 or 128 in q and the caches, not {D} and {Dk}")
+    _refuse(q.dtype in _HALVES and k_cache.dtype == q.dtype and v_cache.dtype == q.dtype, "q and the caches are bf16 or fp16, all the same")
+    _refuse(hkv >= 1 and hq >= 1 and hq % hkv == 0 and hq // hkv <= 128, f"hq={hq} must be a multiple of hkv={hkv}, at most 128 times")
+    _refuse(page in (8, 16, 32, 64, 128), f"page_size={page} must be 8, 16, 32, 64 or 128")
+    _refuse(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
+    _refuse(block_table.dim() == 2 and q_start.dim() == 1 and kv_len.dim() == 1, "block_table is [requests, pages], q_start and kv_len are vectors")
+    R = kv_len.shape[0]
+    _refuse(block_table.shape[0] == R and q_start.shape[0] == R + 1, f"{R} requests: block_table needs as many rows, q_start one more entry")
+    small = (block_table, q_start, kv_len) if tree is None else (block_table, q_start, kv_len, tree)
+    _refuse(all(t.dtype == torch.int32 and t.is_contiguous() for t in small), "block_table, q_start, kv_len and tree are contiguous int32")
+    if tree is None:
+        _refuse(1 <= window < 1 << 31 and 0 <= sinks < 1 << 31, f"window={window} must be positive, sinks={sinks} not negative")
+        words = 0
+    else:
+        _refuse(tree.dim() == 2 and tree.shape[0] == T and (tree.shape[1] >= 1 or T == 0), "tree is [tokens, words]")
+        words = tree.shape[1]
+    scale = D ** -0.5 if scale is None else float(scale)
+    _refuse(0.0 < scale < math.inf, "the scale must be positive and finite")
+    if out is not None:
+        _refuse(out.shape == q.shape and out.dtype == q.dtype, "out has the shape and type of q")
+    for t in (q,) if out is None else (q, out):
+        _refuse(T == 0 or (t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.stride(0) >= 0 and t.stride(1) > 0 and t.data_ptr() % 16 == 0),
+                "the heads of q and out must be contiguous and start at multiples of 16 bytes")
+    device = q.device
+    _refuse(q.is_cuda and all(t.device == device for t in (k_cache, v_cache, *small)) and (out is None or out.device == device) and
+            (status is None or status.device == device), "all tensors must be on one CUDA device")
+    _refuse(status is None or (status.dtype == torch.int32 and status.numel() >= 1), "status is int32")
+    with torch.cuda.device(device):
+        st = stream if stream is not None else torch.cuda.current_stream()
+        with torch.cuda.stream(st):   # what is allocated here belongs to the stream of the call
+            if out is None:
+                out = torch.empty((T, hq, D), dtype=q.dtype, device=device)
+            if T == 0 or R == 0:
+                return out
+            ws_bytes = _C.lib.monofab_masked_attention_ws_bytes(T, hq, hkv, D)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        a = _C.MaskedAttentionArgsC(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
+            None if tree is None else tree.data_ptr(), ws.data_ptr(), None if status is None else status.data_ptr(),
+            q.stride(0), q.stride(1), out.stride(0), out.stride(1), ws_bytes, T, R, hq, hkv, D, page, n_pages, block_table.shape[1], words,
+            0 if tree is not None else window, 0 if tree is not None else sinks, int(q.dtype == torch.float16), scale, 0)
+        _C.check(_C.lib.monofab_masked_attention(ctypes.byref(a), ctypes.c_void_p(st.cuda_stream)))
+    return out
+
+
+def sliding_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window, sinks=0, scale=None, out=None, stream=None, status=None):
+    """Attention over a paged cache within a window, with the first `sinks` keys visible to all: a row at position p sees
+    key j if j <= p and (j > p - window or j < sinks).  Prompts, portions of prompts and single tokens in one ragged batch.
+
+    q [T, hq, D], D 64 or 128, bf16 or fp16, rows and heads at any stride of 16 bytes; k_cache / v_cache
+    [pages, page_size, hkv, D]; block_table int32 [requests, stride]; q_start int32 [requests + 1]: request r's rows are
+    q_start[r] .. q_start[r + 1] - 1; kv_len int32 [requests]: its keys, those of its rows the last of them.  The lengths are read
+    on the device: a call captured in a CUDA graph can be replayed with others.  Returns [T, hq, D] (`out`, which may be q
+    itself): rows that see no key are zeros, rows of no request keep what they hold (are undefined in a new tensor).
+    A bounded wait that ran out is reported in `status` (int32 on the device), or to attention_status().  Keys that some row of
+    a request sees must hold finite values; the others may hold anything."""
+    return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, int(window), int(sinks), None, scale, out, stream, status)
+
+
+def tree_attention(q, k_cache, v_cache, block_table, q_start, kv_len, tree, scale=None, out=None, stream=None, status=None):
+    """Attention of drafted token trees over a paged cache: a request's rows are its drafted tokens, whose keys are the last
+    ones of its kv_len.  A row sees all keys in front of them (the past), and of drafted token d the key if bit d % 32 of
+    tree[row, d // 32] is set.  tree: int32 [T, words] (tree_bits makes it from parents); drafted tokens from 32 * words on
+    are seen by none.  Everything else as in sliding_attention."""
+    return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, 0, 0, tree, scale, out, stream, status)
+
+
+def tree_bits(parents, words=None):
+    """The words of one request's tree for tree_attention, int32 [drafts, words] on the host: parents[i] is the drafted token that
+    token i follows, an earlier one, or -1 where it follows the past.  A token sees itself and what it follows."""
+    seen = []
+    for i, parent in enumerate(parents):
+        _refuse(-1 <= parent < i, f"token {i} cannot follow token {parent}")
+        seen.append((seen[parent] if parent >= 0 else 0) | 1 << i)
+    need = max(1, -(-len(seen) // 32))
+    words = need if words is None else words
+    _refuse(words >= need, f"{len(seen)} drafted tokens need {need} words")
+    signed = [[(b >> 32 * w & 0xffffffff) - (1 << 32 if b >> 32 * w + 31 & 1 else 0) for w in range(words)] for b in seen]
+    return torch.tensor(signed, dtype=torch.int32).reshape(len(seen), words)
+
+
+def attention_status(device=None):
+    """The status bits (include/monofab.h) that sliding_attention and tree_attention calls without a status of their own have left
+    on the device since the last time it was asked.  Waits for the device."""
+    out = ctypes.c_int32()
+    with torch.cuda.device(device):
+        _C.check(_C.lib.monofab_masked_attention_status(ctypes.byref(out)))
+    return out.value

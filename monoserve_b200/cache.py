@@ -1,0 +1,192 @@
+"""Operators on a paged KV cache as launches on a stream: the append of new rows with the norms and the rotation in the
+same pass, pages shared by sequences that fork, pages copied and accepted drafts' rows moved in all layers at once.
+
+The caches are those of the attention (monoserve_b200/attention.py): [pages, page_size, hkv, head_dim], K and V apart, a
+tensor per layer; page 0 is the sink that unused block-table entries point at (monoserve_b200/engine.py:PagePool).  A
+slot is page * page_size + row in the page.  Like every launch, these wait for a resident fabric to stop.
+"""
+import ctypes
+
+import torch
+
+from monoserve_b200 import _C
+from monoserve_b200.attention import _HALVES, _refuse
+from monoserve_b200.engine import PagePool
+
+
+def _stream_of(stream):
+    return ctypes.c_void_p((stream if stream is not None else torch.cuda.current_stream()).cuda_stream)
+
+
+def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, q_out=None, stream=None):
+    """q and k heads of a projection normed and turned, k and v appended to the caches, q returned.
+
+    qkv [T, (hq + 2 hkv) D], bf16 or fp16, rows at any stride of 8 bytes: hq q heads, then hkv k heads, then hkv v heads;
+    k_cache / v_cache [pages, page_size, hkv, D], D 64, 128 or 256; positions, slots int32 [T]; cos_sin fp32
+    [max_pos, rot / 2, 2] (lane_base.rope_table), rot a multiple of 8 up to D; q_norm / k_norm [D] in qkv's type, or None for no
+    norm.  A head x becomes x * rsqrt(mean(x^2) + eps) * norm, and of its first rot dims the pairs (d, d + rot / 2), or
+    (2 d, 2 d + 1) if `interleaved`, are turned by the row of the table of its position (outside the table: the nearest
+    row).  32-bit arithmetic, one rounding.  Slots outside the cache store nothing: -1 for padding.  q_out [T, hq, D] may be the q
+    heads of qkv themselves (qkv.view(T, -1, D)[:, :hq])."""
+    _refuse(qkv.dim() == 2 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "qkv is [T, heads * D], the caches are [pages, page_size, hkv, D]")
+    T = qkv.shape[0]
+    n_pages, page, hkv, D = k_cache.shape
+    _refuse(D in (64, 128, 256), f"head_dim must be 64, 128 or 256, not {D}")
+    _refuse(hq >= 1 and qkv.shape[1] == (hq + 2 * hkv) * D, f"qkv has {qkv.shape[1]} columns, not those of {hq} + 2 * {hkv} heads of {D}")
+    _refuse(qkv.dtype in _HALVES and k_cache.dtype == qkv.dtype and v_cache.dtype == qkv.dtype, "qkv and the caches are bf16 or fp16, all the same")
+    _refuse(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
+    _refuse(n_pages * page < 1 << 31, "the caches have more slots than int32 can name")
+    _refuse(all(t.dim() == 1 and t.shape[0] == T and t.dtype == torch.int32 and t.is_contiguous() for t in (positions, slots)), "positions and slots are int32 [T]")
+    _refuse(cos_sin.dim() == 3 and cos_sin.shape[2] == 2 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous(), "cos_sin is fp32 [max_pos, rot / 2, 2]")
+    rot = 2 * cos_sin.shape[1]
+    _refuse(cos_sin.shape[0] >= 1 and rot % 8 == 0 and rot <= D, f"rot={rot} must be a multiple of 8 up to {D}")
+    norms = [w for w in (q_norm, k_norm) if w is not None]
+    _refuse(all(w.shape == (D,) and w.dtype == qkv.dtype and w.is_contiguous() for w in norms), "q_norm and k_norm are [D] in the type of qkv")
+    _refuse(eps >= 0, "eps must not be negative")
+    _refuse(T == 0 or (qkv.stride(1) == 1 and qkv.stride(0) % 4 == 0 and qkv.stride(0) >= qkv.shape[1] * (T > 1)), "rows of qkv must be contiguous and start at multiples of 8 bytes")
+    if q_out is not None:
+        _refuse(q_out.shape == (T, hq, D) and q_out.dtype == qkv.dtype and q_out.stride(2) == 1 and (hq == 1 or q_out.stride(1) == D) and
+                q_out.stride(0) % 4 == 0 and (T <= 1 or q_out.stride(0) >= hq * D), "q_out is [T, hq, D] with contiguous rows that start at multiples of 8 bytes")
+    device = qkv.device
+    _refuse(qkv.is_cuda and all(t.device == device for t in (k_cache, v_cache, positions, slots, cos_sin, *norms, *(() if q_out is None else (q_out,)))),
+            "all tensors must be on one CUDA device")
+    with torch.cuda.device(device):
+        st = stream if stream is not None else torch.cuda.current_stream()
+        if q_out is None:
+            with torch.cuda.stream(st):
+                q_out = torch.empty((T, hq, D), dtype=qkv.dtype, device=device)
+        _C.check(_C.lib.monofab_qk_rope(
+            qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
+            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), q_out.data_ptr(), q_out.stride(0),
+            k_cache.data_ptr(), v_cache.data_ptr(), n_pages * page, T, hq, hkv, D, rot, int(bool(interleaved)), int(qkv.dtype == torch.float16),
+            float(eps), ctypes.c_void_p(st.cuda_stream)))
+    return q_out
+
+
+class SharedPages(PagePool):
+    """A page pool whose pages several sequences can hold: a page is free again when as many have given it as had it."""
+
+    def __init__(self, n_pages):
+        super().__init__(n_pages)
+        self.n_pages = n_pages
+        self.holders = [0] * n_pages
+
+    def take(self, n):
+        pages = super().take(n)
+        for p in pages:
+            self.holders[p] = 1
+        return pages
+
+    def share(self, pages):
+        """Another sequence holds these pages, too."""
+        _refuse(all(0 < p < self.n_pages and self.holders[p] > 0 for p in pages), "only pages that a sequence holds can be shared")
+        for p in pages:
+            self.holders[p] += 1
+        return list(pages)
+
+    def give(self, pages):
+        """A sequence lets go of these pages.  Nothing changes where one of them is not held."""
+        left = {}
+        for p in pages:
+            _refuse(0 < p < self.n_pages and left.setdefault(p, self.holders[p]) > 0, f"page {p} is held by no sequence")
+            left[p] -= 1
+        for p, n in left.items():
+            self.holders[p] = n
+        super().give([p for p in dict.fromkeys(pages) if left[p] == 0])
+
+    def fork(self, pages, length, page_size):
+        """The pages of a new sequence that starts as the first `length` tokens of one with these pages, and the copies
+        [(from, to)] to make for it: it shares the full pages, and gets its own copy of the one that it will go on filling."""
+        full, rest = divmod(length, page_size)
+        _refuse(0 <= length <= len(pages) * page_size, f"{length} tokens in {len(pages)} pages of {page_size}")
+        own = self.take(1) if rest else []
+        return self.share(pages[:full]) + own, [(pages[full], p) for p in own]
+
+    def compact(self, sequences):
+        """Moves held pages to the lowest numbers.  sequences: lists of pages, all that are held; their entries are
+        replaced.  Returns the copies [(from, to)] to make before anybody reads the new pages."""
+        seen = [0] * self.n_pages
+        for pages in sequences:
+            for p in pages:
+                _refuse(0 < p < self.n_pages, f"page {p} is no page of the pool")
+                seen[p] += 1
+        _refuse(seen == self.holders, "compact needs the pages of every sequence that holds some")
+        held = [p for p in range(1, self.n_pages) if self.holders[p]]
+        holes = [p for p in range(1, len(held) + 1) if not self.holders[p]]
+        moves = dict(zip([p for p in held if p > len(held)], holes))
+        for pages in sequences:
+            pages[:] = [moves.get(p, p) for p in pages]
+        for a, b in moves.items():
+            self.holders[b], self.holders[a] = self.holders[a], 0
+        self.free = list(range(self.n_pages - 1, len(held), -1))
+        return list(moves.items())
+
+
+class CachePages:
+    """The cache tensors of all layers as one object whose pages and rows are moved together, one launch for all of them.
+
+    pages = CachePages(kv.k + kv.v)      # [pages, page_size, hkv, D] each, kept alive and in place by the caller
+    pages.copy(src, dst); pages.accept(block_table, base, path, count); pages.check()
+    """
+
+    def __init__(self, tensors):
+        tensors = list(tensors)
+        _refuse(tensors and all(t.dim() == 4 for t in tensors), "cache tensors are [pages, page_size, hkv, D]")
+        t0 = tensors[0]
+        _refuse(all(t.shape == t0.shape and t.dtype == t0.dtype and t.device == t0.device and t.is_contiguous() for t in tensors),
+                "cache tensors must be contiguous and have one shape, type and device")
+        self.n_pages, self.page_size = t0.shape[:2]
+        self.row_bytes = t0.shape[2] * t0.shape[3] * t0.element_size()
+        _refuse(self.n_pages >= 1 and self.page_size >= 1 and self.row_bytes >= 16 and self.row_bytes % 16 == 0 and all(t.data_ptr() % 16 == 0 for t in tensors),
+                "rows of a cache tensor must be multiples of 16 bytes")
+        _refuse(len(tensors) <= 65535 and len({t.data_ptr() for t in tensors}) == len(tensors), "at most 65535 cache tensors, each of them once")
+        _refuse(t0.is_cuda, "cache tensors must be on a CUDA device")
+        self.tensors, self.device = tensors, t0.device
+        self._table = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64).to(self.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        torch.cuda.current_stream(self.device).synchronize()   # both are there for calls on any stream
+
+    def _indexes(self, name, t, *shape):
+        if not isinstance(t, torch.Tensor):
+            t = torch.tensor(t, dtype=torch.int32).reshape(shape).to(self.device)
+        _refuse(t.dtype == torch.int32 and t.is_contiguous() and t.device == self.device and t.dim() == len(shape) and
+                all(s in (-1, n) for s, n in zip(shape, t.shape)), f"{name} is int32 on the device of the cache, of shape {list(shape)}")
+        return t
+
+    def copy(self, src, dst, stream=None):
+        """Page dst[i] takes what page src[i] holds, in all tensors.  src, dst: int32 tensors on the device, or host lists.  One page
+        may go to many, but a destination may be no other pair's source or destination: lists are refused, of tensors such
+        pairs (and pages that do not exist) are left out, which check() tells."""
+        if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
+            src, dst = list(src), list(dst)
+            _refuse(len(src) == len(dst) and all(0 <= p < self.n_pages for p in src + dst), "src and dst are as many page numbers of the cache")
+            pairs = [(s, d) for s, d in zip(src, dst) if s != d]
+            src, dst = [s for s, _ in pairs], [d for _, d in pairs]
+            _refuse(len(set(dst)) == len(dst) and not set(dst) & set(src), "a destination is another pair's source or destination")
+        with torch.cuda.device(self.device), torch.cuda.stream(stream):
+            src = self._indexes("src", src, -1)
+            dst = self._indexes("dst", dst, src.shape[0])
+            _refuse(src.shape[0] <= 65535, "at most 65535 pages a call")
+            _C.check(_C.lib.monofab_page_copy(self._table.data_ptr(), len(self.tensors), src.data_ptr(), dst.data_ptr(), src.shape[0], self.n_pages,
+                                              self.page_size * self.row_bytes, self.status.data_ptr(), _stream_of(stream)))
+
+    def accept(self, block_table, base, path, count, stream=None):
+        """The rows of accepted drafts move to the places behind their sequence, in all tensors: of request r, row base[r] + path[r, i]
+        to row base[r] + i for i < count[r], as they were before the call.  block_table int32 [requests, stride], base and
+        count int32 [requests], path int32 [requests, most <= 2048], on the device.  Rows in places that do not exist stay,
+        which check() tells.  Requests must not share the pages of these rows."""
+        block_table = self._indexes("block_table", block_table, -1, -1)
+        R = block_table.shape[0]
+        base, count, path = self._indexes("base", base, R), self._indexes("count", count, R), self._indexes("path", path, R, -1)
+        _refuse(path.shape[1] <= 2048 and R <= 65535 and block_table.shape[1] >= 1, "at most 2048 rows of a path, 65535 requests")
+        with torch.cuda.device(self.device):
+            _C.check(_C.lib.monofab_accept_rows(self._table.data_ptr(), len(self.tensors), block_table.data_ptr(), block_table.shape[1], base.data_ptr(),
+                                                path.data_ptr(), count.data_ptr(), R, path.shape[1], self.page_size, self.n_pages, self.row_bytes,
+                                                self.status.data_ptr(), _stream_of(stream)))
+
+    def check(self):
+        """Raises if a copy or an accept since the last check left something out.  Waits for the device."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            raise RuntimeError(f"monofab: pages or rows were left out, status {bits}")

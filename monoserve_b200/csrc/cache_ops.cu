@@ -1,0 +1,372 @@
+// Operators on a paged KV cache, launched on a stream: the append of new rows (norms of queries and keys for each head
+// and the position rotation in the same pass), copies of whole pages in all layers, and the move of accepted drafts'
+// rows to the places behind their sequence in all layers.
+//
+// A cache tensor is [pages][page size][kv heads][head dim], 16-bit values; a slot is page * page size + row in the page.
+// All of this is bound by HBM (or, for a few rows, by the latency of one launch): every kernel keeps several 16-byte
+// (or paired 8-byte) accesses a thread in flight and touches each byte once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "moe_layer.h"
+
+namespace mf {
+
+namespace {
+
+template <class E>
+struct Pack;
+template <>
+struct Pack<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 open(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+  static __device__ __forceinline__ uint32_t close(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Pack<__half> {
+  static __device__ __forceinline__ float2 open(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+  static __device__ __forceinline__ uint32_t close(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+struct QkRopeParams {
+  const uint16_t* qkv;      // [T] rows of (hq + 2 hkv) heads, `ld` values apart
+  const int32_t* positions; // [T]
+  const int32_t* slots;     // [T]
+  const float* cos_sin;     // [max_pos][rot / 2][2]
+  const uint16_t *q_norm, *k_norm;   // [D] or null: no norm
+  uint16_t* q_out;          // [T] rows of hq heads, `ld_out` values apart
+  uint16_t *k_cache, *v_cache;
+  long long ld, ld_out, n_slots;
+  int T, hq, hkv, rot, max_pos, interleaved;
+  float eps;
+};
+
+// A lane holds two runs of four dims of a head, `a` and `b`, so that both values of a rotated pair are its own whatever
+// the pairs are: of the first rot / 8 lanes, halves: dims 4 l.. of either half; neighbours: dims 8 l.. and 8 l + 4..; both
+// take the four (cos, sin) from 4 l on. The other lanes hold what is not turned, in order. So there is no exchange but the
+// sum of squares. A unit is U passes of a warp over the heads of one row (32 / (D / 8) heads a pass): their loads are issued
+// together, and the row's (cos, sin) and the norm weights are read once for all of them.
+// Everything is in 32 bits and rounded once, at the store.
+// 8191 rows of 40 heads of 128 (168 MB): see the table of times in the documents; bound by HBM.
+template <class E, int D, int U, bool kNeighbours>
+__global__ void __launch_bounds__(256) qk_rope_kernel(const __grid_constant__ QkRopeParams p) {
+  constexpr int kLanes = D / 8, kHeads = 32 / kLanes;
+  chain_release();
+  const int lane = threadIdx.x & 31, l = lane % kLanes;
+  const int heads = p.hq + 2 * p.hkv, units = (heads + U * kHeads - 1) / (U * kHeads);
+  const long long unit = static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
+  const long long row = unit / units;
+  chain_wait();
+  if (row >= p.T) return;   // the whole warp
+  const int head0 = static_cast<int>(unit - row * units) * U * kHeads + lane / kLanes;
+  const bool turns = l < p.rot / 8;
+  const int da = turns && !kNeighbours ? 4 * l : 8 * l;
+  const int db = turns && !kNeighbours ? p.rot / 2 + 4 * l : 8 * l + 4;
+  const uint16_t* const from = p.qkv + row * p.ld;
+  uint2 a[U], b[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int head = head0 + u * kHeads;
+    if (head < heads) {
+      a[u] = *reinterpret_cast<const uint2*>(from + head * D + da);
+      b[u] = *reinterpret_cast<const uint2*>(from + head * D + db);
+    } else {
+      a[u] = b[u] = make_uint2(0, 0);
+    }
+  }
+  const int slot = p.slots[row];
+  float4 cs[2] = {make_float4(1.f, 0.f, 1.f, 0.f), make_float4(1.f, 0.f, 1.f, 0.f)};   // (cos, sin) of four pairs
+  if (turns) {
+    const int pos = max(0, min(p.positions[row], p.max_pos - 1));
+    const float4* const t = reinterpret_cast<const float4*>(p.cos_sin + (static_cast<long long>(pos) * (p.rot / 2) + 4 * l) * 2);
+    cs[0] = t[0];
+    cs[1] = t[1];
+  }
+  uint2 w[2][2];   // norm weights of q and of k heads
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint16_t* const n = i ? p.k_norm : p.q_norm;
+    w[i][0] = n ? *reinterpret_cast<const uint2*>(n + da) : make_uint2(0, 0);
+    w[i][1] = n ? *reinterpret_cast<const uint2*>(n + db) : make_uint2(0, 0);
+  }
+  const bool stored = slot >= 0 && slot < p.n_slots;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int head = head0 + u * kHeads;
+    const bool is_q = head < p.hq, is_k = !is_q && head < p.hq + p.hkv;
+    float x[8];
+    {
+      const float2 t0 = Pack<E>::open(a[u].x), t1 = Pack<E>::open(a[u].y), t2 = Pack<E>::open(b[u].x), t3 = Pack<E>::open(b[u].y);
+      x[0] = t0.x, x[1] = t0.y, x[2] = t1.x, x[3] = t1.y, x[4] = t2.x, x[5] = t2.y, x[6] = t3.x, x[7] = t3.y;
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int bit = kLanes / 2; bit >= 1; bit >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, bit);
+    if (head >= heads) continue;
+    uint16_t* to;
+    if (is_q) {
+      to = p.q_out + row * p.ld_out + head * D;
+    } else {
+      if (!stored) continue;
+      const int kvh = is_k ? head - p.hq : head - p.hq - p.hkv;
+      to = (is_k ? p.k_cache : p.v_cache) + (static_cast<long long>(slot) * p.hkv + kvh) * D;
+    }
+    uint2 ra = a[u], rb = b[u];
+    if (is_q || is_k) {
+      if (is_q ? p.q_norm != nullptr : p.k_norm != nullptr) {
+        const float inv = rsqrtf(ss / D + p.eps);
+        const uint2 wa = is_q ? w[0][0] : w[1][0], wb = is_q ? w[0][1] : w[1][1];
+        const float2 t0 = Pack<E>::open(wa.x), t1 = Pack<E>::open(wa.y), t2 = Pack<E>::open(wb.x), t3 = Pack<E>::open(wb.y);
+        const float v[8] = {t0.x, t0.y, t1.x, t1.y, t2.x, t2.y, t3.x, t3.y};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * v[i];
+      }
+      if (turns) {
+        const float c[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i0 = kNeighbours ? 2 * j : j, i1 = kNeighbours ? 2 * j + 1 : j + 4;
+          const float first = x[i0], second = x[i1];
+          x[i0] = first * c[2 * j] - second * c[2 * j + 1];
+          x[i1] = second * c[2 * j] + first * c[2 * j + 1];
+        }
+      }
+      ra = make_uint2(Pack<E>::close(x[0], x[1]), Pack<E>::close(x[2], x[3]));
+      rb = make_uint2(Pack<E>::close(x[4], x[5]), Pack<E>::close(x[6], x[7]));
+    }
+    *reinterpret_cast<uint2*>(to + da) = ra;
+    *reinterpret_cast<uint2*>(to + db) = rb;
+  }
+}
+
+template <class E, int D>
+cudaError_t launch_qk_rope(const QkRopeParams& p, cudaStream_t stream) {
+  constexpr int kHeads = 32 / (D / 8);
+  const int heads = p.hq + 2 * p.hkv;
+  auto go = [&](auto kernel, int u) {
+    const long long units = static_cast<long long>(p.T) * ((heads + u * kHeads - 1) / (u * kHeads));
+    return launch_chained(kernel, dim3(static_cast<unsigned>((units + 7) / 8)), dim3(256), 0, stream, p);
+  };
+  return p.interleaved ? go(qk_rope_kernel<E, D, 4, true>, 4) : go(qk_rope_kernel<E, D, 4, false>, 4);
+}
+
+// ------------------------------------------------------------------------------------------------- pages and rows
+
+struct PageCopyParams {
+  const unsigned long long* tensors;   // [n_tensors] device addresses
+  const int32_t *src, *dst;
+  int* status;
+  int n_tensors, pairs, n_pages, chunks, per_block;   // chunks of a page, tensors of a block
+  long long page_bytes;
+};
+
+constexpr int kCopyThreads = 256, kCopyLoads = 4, kCopyBytes = kCopyThreads * kCopyLoads * 16;
+
+// Block (chunk of a page, group of tensors, pair). Whether the pair may be copied is looked at first, in every block alike:
+// its destination may be no other pair's source or destination, and its source no other pair's destination - copies run side
+// by side, and either would make the result depend on their order.
+__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_constant__ PageCopyParams p) {
+  chain_release();
+  chain_wait();
+  const int pair = blockIdx.z;
+  const int src = p.src[pair], dst = p.dst[pair];
+  bool bad = src < 0 || src >= p.n_pages || dst < 0 || dst >= p.n_pages;
+  for (int j = threadIdx.x; j < p.pairs; j += kCopyThreads) {
+    if (j == pair) continue;
+    const int s = p.src[j], d = p.dst[j];
+    bad = bad || s == dst || d == dst || d == src;
+  }
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) atomicOr(p.status, kErrBadArgs);
+    return;
+  }
+  if (src == dst) return;
+  const long long at = static_cast<long long>(blockIdx.x) * kCopyBytes + threadIdx.x * 16;
+  const int first = blockIdx.y * p.per_block, last = min(first + p.per_block, p.n_tensors);
+  for (int t = first; t < last; ++t) {
+    char* const base = reinterpret_cast<char*>(p.tensors[t]);
+    const char* const from = base + src * p.page_bytes + at;
+    char* const to = base + dst * p.page_bytes + at;
+    uint4 v[kCopyLoads];
+#pragma unroll
+    for (int i = 0; i < kCopyLoads; ++i)
+      if (at + i * (kCopyThreads * 16) < p.page_bytes) v[i] = *reinterpret_cast<const uint4*>(from + i * (kCopyThreads * 16));
+#pragma unroll
+    for (int i = 0; i < kCopyLoads; ++i)
+      if (at + i * (kCopyThreads * 16) < p.page_bytes) *reinterpret_cast<uint4*>(to + i * (kCopyThreads * 16)) = v[i];
+  }
+}
+
+struct AcceptParams {
+  const unsigned long long* tensors;
+  const int32_t *block_table, *base, *path, *count;
+  int* status;
+  int n_tensors, requests, most, bt_stride, page, n_pages;
+  int lanes;           // 16-byte pieces of a row that a block moves, a power of two
+  int pieces;          // of a row
+};
+
+constexpr int kAcceptThreads = 256, kAcceptRows = 8;   // rows a thread holds
+
+// Block (slice of a row, tensor, request): every row that moves is read before the first is written, so a path may lead
+// anywhere among the drafts, whatever it overwrites. The slice is as wide as lets the block's threads hold all rows.
+__global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptParams p) {
+  chain_release();
+  chain_wait();
+  const int r = blockIdx.z;
+  const int n = max(0, min(p.count[r], p.most));
+  const long long base = p.base[r];
+  const int piece = blockIdx.x * p.lanes + threadIdx.x % p.lanes;
+  const int row0 = threadIdx.x / p.lanes, step = kAcceptThreads / p.lanes;
+  char* const tensor = reinterpret_cast<char*>(p.tensors[blockIdx.y]);
+  const int32_t* const table = p.block_table + static_cast<long long>(r) * p.bt_stride;
+  bool bad = false;
+  auto address = [&](long long at) -> char* {
+    if (at < 0 || at >= static_cast<long long>(p.bt_stride) * p.page) return nullptr;
+    const int page = table[at / p.page];
+    if (page < 0 || page >= p.n_pages) return nullptr;
+    return tensor + ((static_cast<long long>(page) * p.page + at % p.page) * p.pieces + piece) * 16;
+  };
+  uint4 v[kAcceptRows];
+  char* to[kAcceptRows];
+#pragma unroll
+  for (int i = 0; i < kAcceptRows; ++i) {
+    const int row = row0 + i * step;
+    to[i] = nullptr;
+    if (row >= n) continue;
+    const int from_row = p.path[static_cast<long long>(r) * p.most + row];
+    const char* const from = from_row < 0 ? nullptr : address(base + from_row);
+    char* const dst = address(base + row);
+    if (!from || !dst) {
+      bad = true;
+      continue;
+    }
+    if (from == dst || piece >= p.pieces) continue;
+    v[i] = *reinterpret_cast<const uint4*>(from);
+    to[i] = dst;
+  }
+  if (bad) atomicOr(p.status, kErrBadArgs);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kAcceptRows; ++i)
+    if (to[i]) *reinterpret_cast<uint4*>(to[i]) = v[i];
+}
+
+}  // namespace
+
+}  // namespace mf
+
+using namespace mf;
+
+extern "C" int monofab_qk_rope(const void* qkv, int64_t ld_qkv, const int32_t* positions, const int32_t* slots,
+                               const float* cos_sin, int max_pos, const void* q_norm, const void* k_norm, void* q_out,
+                               int64_t ld_out, void* k_cache, void* v_cache, int64_t n_slots, int T, int hq, int hkv,
+                               int head_dim, int rot, int interleaved, int fp16, float eps, void* stream) {
+  if (T < 0) return fail(MONOFAB_EINVAL, "qk_rope: negative T");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(MONOFAB_EINVAL, "qk_rope: head_dim=%d must be 64, 128 or 256", head_dim);
+  if (hq < 0 || hkv < 0 || hq + hkv < 1 || hq > (1 << 20) || hkv > (1 << 20)) return fail(MONOFAB_EINVAL, "qk_rope: hq=%d, hkv=%d", hq, hkv);
+  if (rot < 0 || rot > head_dim || rot % 8) return fail(MONOFAB_EINVAL, "qk_rope: rot=%d must be a multiple of 8 up to head_dim", rot);
+  if (T == 0) return MONOFAB_OK;
+  if (!qkv || !positions || !slots || (rot && !cos_sin) || (hq && !q_out) || (hkv && (!k_cache || !v_cache)))
+    return fail(MONOFAB_EINVAL, "qk_rope: NULL argument");
+  if (max_pos < 1 || n_slots < 0) return fail(MONOFAB_EINVAL, "qk_rope: max_pos=%d, n_slots=%lld", max_pos, static_cast<long long>(n_slots));
+  if (!(eps >= 0.f)) return fail(MONOFAB_EINVAL, "qk_rope: eps must not be negative");
+  const uintptr_t at8 = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_cache) |
+                        reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(q_norm) | reinterpret_cast<uintptr_t>(k_norm);
+  if ((at8 & 7) || (reinterpret_cast<uintptr_t>(cos_sin) & 15) || (ld_qkv & 3) || (ld_out & 3))
+    return fail(MONOFAB_EINVAL, "qk_rope: rows must start at multiples of 8 bytes, the table at one of 16");
+  QkRopeParams p{};
+  p.qkv = static_cast<const uint16_t*>(qkv);
+  p.positions = positions;
+  p.slots = slots;
+  p.cos_sin = cos_sin;
+  p.q_norm = static_cast<const uint16_t*>(q_norm);
+  p.k_norm = static_cast<const uint16_t*>(k_norm);
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.k_cache = static_cast<uint16_t*>(k_cache);
+  p.v_cache = static_cast<uint16_t*>(v_cache);
+  p.ld = ld_qkv;
+  p.ld_out = ld_out;
+  p.n_slots = n_slots;
+  p.T = T;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.rot = rot;
+  p.max_pos = max_pos;
+  p.interleaved = interleaved != 0;
+  p.eps = eps;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto e) {
+    using E = decltype(e);
+    return head_dim == 64 ? launch_qk_rope<E, 64>(p, st) : head_dim == 128 ? launch_qk_rope<E, 128>(p, st) : launch_qk_rope<E, 256>(p, st);
+  };
+  MF_CUDA(fp16 ? go(__half()) : go(__nv_bfloat16()));
+  return MONOFAB_OK;
+}
+
+extern "C" int monofab_page_copy(const uint64_t* tensors, int n_tensors, const int32_t* src, const int32_t* dst, int pairs,
+                                 int n_pages, int64_t page_bytes, int32_t* status, void* stream) {
+  if (n_tensors < 1 || pairs < 0 || n_pages < 1) return fail(MONOFAB_EINVAL, "page_copy: n_tensors=%d, pairs=%d, n_pages=%d", n_tensors, pairs, n_pages);
+  if (page_bytes < 16 || page_bytes % 16) return fail(MONOFAB_EINVAL, "page_copy: page_bytes=%lld must be a multiple of 16", static_cast<long long>(page_bytes));
+  if (pairs == 0) return MONOFAB_OK;
+  if (!tensors || !src || !dst || !status) return fail(MONOFAB_EINVAL, "page_copy: NULL argument");
+  if (pairs > 65535) return fail(MONOFAB_EINVAL, "page_copy: %d pairs, at most 65535 a call", pairs);
+  PageCopyParams p{};
+  p.tensors = reinterpret_cast<const unsigned long long*>(tensors);
+  p.src = src;
+  p.dst = dst;
+  p.status = status;
+  p.n_tensors = n_tensors;
+  p.pairs = pairs;
+  p.n_pages = n_pages;
+  p.page_bytes = page_bytes;
+  p.per_block = 1;
+  const long long chunks = (page_bytes + kCopyBytes - 1) / kCopyBytes;
+  if (chunks > 65535 || n_tensors > 65535) return fail(MONOFAB_EINVAL, "page_copy: pages of %lld bytes in %d tensors", static_cast<long long>(page_bytes), n_tensors);
+  MF_CUDA(launch_chained(page_copy_kernel, dim3(static_cast<unsigned>(chunks), (n_tensors + p.per_block - 1) / p.per_block, pairs),
+                         dim3(kCopyThreads), 0, static_cast<cudaStream_t>(stream), p));
+  return MONOFAB_OK;
+}
+
+extern "C" int monofab_accept_rows(const uint64_t* tensors, int n_tensors, const int32_t* block_table, int bt_stride,
+                                   const int32_t* base, const int32_t* path, const int32_t* count, int requests, int most,
+                                   int page_size, int n_pages, int64_t row_bytes, int32_t* status, void* stream) {
+  if (n_tensors < 1 || n_tensors > 65535 || requests < 0 || most < 0 || page_size < 1 || n_pages < 1 || bt_stride < 1)
+    return fail(MONOFAB_EINVAL, "accept_rows: bad sizes");
+  if (row_bytes < 16 || row_bytes % 16 || row_bytes > (1 << 20))
+    return fail(MONOFAB_EINVAL, "accept_rows: row_bytes=%lld must be a multiple of 16 up to 2^20", static_cast<long long>(row_bytes));
+  if (requests > 65535) return fail(MONOFAB_EINVAL, "accept_rows: %d requests, at most 65535 a call", requests);
+  if (most > kAcceptThreads * kAcceptRows) return fail(MONOFAB_EINVAL, "accept_rows: paths of %d rows, at most %d", most, kAcceptThreads * kAcceptRows);
+  if (requests == 0 || most == 0) return MONOFAB_OK;
+  if (!tensors || !block_table || !base || !path || !count || !status) return fail(MONOFAB_EINVAL, "accept_rows: NULL argument");
+  AcceptParams p{};
+  p.tensors = reinterpret_cast<const unsigned long long*>(tensors);
+  p.block_table = block_table;
+  p.base = base;
+  p.path = path;
+  p.count = count;
+  p.status = status;
+  p.n_tensors = n_tensors;
+  p.requests = requests;
+  p.most = most;
+  p.bt_stride = bt_stride;
+  p.page = page_size;
+  p.n_pages = n_pages;
+  p.pieces = static_cast<int>(row_bytes / 16);
+  p.lanes = 1;
+  while (2 * p.lanes <= kAcceptThreads && 2 * p.lanes * most <= kAcceptThreads * kAcceptRows && p.lanes < p.pieces) p.lanes *= 2;
+  MF_CUDA(launch_chained(accept_kernel, dim3((p.pieces + p.lanes - 1) / p.lanes, n_tensors, requests), dim3(kAcceptThreads), 0,
+                         static_cast<cudaStream_t>(stream), p));
+  return MONOFAB_OK;
+}

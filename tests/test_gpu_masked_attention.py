@@ -1,0 +1,252 @@
+"""sliding_attention and tree_attention against the formula in 64 bits (tests/masked_attention_cases.py), at the lengths,
+masks, strides and orders where they can go wrong."""
+import pytest
+import torch
+
+from tests.masked_attention_cases import make, reference, sliding_mask, tolerance, tree_mask
+
+pytestmark = pytest.mark.gpu
+BF, FP = torch.bfloat16, torch.float16
+
+
+def on_gpu(*tensors):
+    return [t.cuda() for t in tensors]
+
+
+def run_sliding(batch, window, sinks, **kw):
+    from monoserve_b200.attention import sliding_attention
+    return sliding_attention(*on_gpu(*batch), window, sinks=sinks, **kw)
+
+
+def check(out, batch, masks, scale=None):
+    from monoserve_b200.attention import attention_status
+    assert attention_status() == 0
+    ref, weighted = reference(*batch, masks, scale=scale)
+    tol = tolerance(ref, weighted, batch[0].dtype, int(batch[5].max()))
+    err = (out.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+def sliding_masks(batch, window, sinks):
+    start, kv = batch[4].tolist(), batch[5].tolist()
+    return [sliding_mask(b - a, L, window, sinks) for a, b, L in zip(start, start[1:], kv)]
+
+
+HEADS = [(32, 4), (12, 4), (6, 6), (12, 1)]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_sliding_ragged_batch(dtype, dim, hq, hkv):
+    """Prompts, portions and single tokens together, windows and sinks inside, at and across the 128-key tiles."""
+    batch = make([1, 5, 0, 33, 130, 1], [0, 700, 50, 3, 260, 2049], hq, hkv, dim, 16, dtype, seed=hq + dim)
+    for window, sinks in ((1, 0), (7, 3), (128, 0), (129, 130), (500, 17), (1 << 31 - 1, 0)):
+        check(run_sliding(batch, window, sinks), batch, sliding_masks(batch, window, sinks))
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128])
+def test_sliding_single_tokens_of_all_lengths(page):
+    past = [0, 1, 15, 126, 127, 128, 129, 255, 256, 1000, 4095, 9000]
+    batch = make([1] * len(past), past, 32, 4, 128, page, BF, seed=page)
+    for window, sinks in ((4096, 4), (1024, 0), (100000, 0), (200, 300)):
+        check(run_sliding(batch, window, sinks), batch, sliding_masks(batch, window, sinks))
+
+
+@pytest.mark.parametrize("window,sinks", [(1024, 4), (100000, 0), (130, 600)])
+def test_sliding_long_prompts(window, sinks):
+    batch = make([1500, 777], [0, 901], 32, 4, 128, 16, BF, seed=5)
+    check(run_sliding(batch, window, sinks), batch, sliding_masks(batch, window, sinks))
+
+
+def test_one_long_context():
+    """A context long enough to be split over every SM."""
+    batch = make([1], [100_000], 8, 1, 128, 64, BF, seed=6)
+    for window, sinks in ((1 << 30, 0), (70_001, 129)):
+        check(run_sliding(batch, window, sinks), batch, sliding_masks(batch, window, sinks))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_no_row_sees_may_hold_anything(dim):
+    """Keys between the sinks and the window, behind the last one and in other pages are NaN; so are pages nobody owns."""
+    batch = make([1, 3, 40], [300, 900, 513], 32, 4, dim, 16, BF, seed=7, fill=float("nan"))
+    q, kc, vc, bt, start, kv = batch
+    window, sinks = 70, 5
+    for r, (a, b, L) in enumerate(zip(start.tolist(), start.tolist()[1:], kv.tolist())):
+        for j in range(sinks, L - (b - a) - window + 1):
+            kc[bt[r, j // 16], j % 16] = float("nan")
+            vc[bt[r, j // 16], j % 16] = float("inf")
+    check(run_sliding(batch, window, sinks), batch, sliding_masks(batch, window, sinks))
+
+
+def test_rows_that_see_nothing_and_rows_of_nobody():
+    """More rows than keys: the rows in front of the first key are zeros; rows behind the last request are left alone, those
+    of requests without keys are zeros."""
+    from monoserve_b200.attention import sliding_attention
+    q, kc, vc, bt, start, kv = make([6, 2, 4], [10, 0, 20], 32, 4, 128, 16, BF, seed=8)
+    kv = torch.tensor([4, 0, 24], dtype=torch.int32)
+    q = torch.cat([q, q[:3]])
+    out = torch.full_like(q, 7.0).cuda()
+    args = on_gpu(q, kc, vc, bt, start, kv)
+    sliding_attention(*args, 100, out=out)
+    masks = [sliding_mask(6, 4, 100, 0), torch.zeros(2, 0, dtype=torch.bool), sliding_mask(4, 24, 100, 0)]
+    batch = (q[:12], kc, vc, bt, start, kv)
+    check(out[:12], batch, masks)
+    assert bool((out[:2] == 0).all()) and bool((out[6:8] == 0).all()) and bool((out[12:] == 7).all())
+
+
+def test_keys_end_with_the_block_table():
+    batch = make([2], [62], 4, 4, 64, 16, BF, seed=9)
+    q, kc, vc, bt, start, kv = batch
+    kv = kv + 30   # 94 keys said, 64 there: the rows are at positions 92 and 93
+    batch = (q, kc, vc, bt, start, kv)
+    check(run_sliding(batch, 40, 3), batch, sliding_masks(batch, 40, 3))
+    check(run_sliding(batch, 20, 0), batch, sliding_masks(batch, 20, 0))
+
+
+def random_trees(rows, seed, empty=False):
+    g = torch.Generator().manual_seed(seed)
+    words = max(1, -(-max(rows) // 32))
+    t = torch.randint(-(1 << 31), 1 << 31, (sum(rows), words), generator=g).to(torch.int32)
+    if empty:
+        t[::2] = 0
+    return t
+
+
+def tree_masks(batch, tree):
+    start, kv = batch[4].tolist(), batch[5].tolist()
+    return [tree_mask(tree[a:b], b - a, L) for a, b, L in zip(start, start[1:], kv)]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_tree_any_bits(dtype, dim, hq, hkv):
+    """Any bits, also those of later tokens; drafted tokens that begin anywhere in a tile of keys; rows that see nothing."""
+    from monoserve_b200.attention import tree_attention
+    rows, past = [1, 8, 33, 64, 100, 7, 0], [0, 127, 250, 1000, 128, 0, 40]
+    batch = make(rows, past, hq, hkv, dim, 16, dtype, seed=hq * dim)
+    for empty in (False, True):
+        tree = random_trees(rows, hq, empty)
+        check(tree_attention(*on_gpu(*batch), tree.cuda()), batch, tree_masks(batch, tree))
+
+
+def test_tree_of_parents_and_few_words():
+    from monoserve_b200.attention import tree_attention, tree_bits
+    parents = [-1, 0, 0, 1, 1, 2, -1, 6] + list(range(7, 39))
+    bits = tree_bits(parents)
+    assert bits.shape == (40, 2)
+    batch = make([40], [333], 32, 4, 128, 16, BF, seed=11)
+    check(tree_attention(*on_gpu(*batch), bits.cuda()), batch, tree_masks(batch, bits))
+    short = bits[:, :1].contiguous()   # drafted tokens from 32 on are seen by none
+    check(tree_attention(*on_gpu(*batch), short.cuda()), batch, tree_masks(batch, short))
+
+
+def test_a_chain_is_causal_attention():
+    from monoserve_b200.attention import sliding_attention, tree_attention, tree_bits
+    batch = on_gpu(*make([16, 16], [500, 77], 32, 4, 128, 16, BF, seed=12))
+    chain = torch.cat([tree_bits(range(-1, 15))] * 2).cuda()
+    assert torch.equal(tree_attention(*batch, chain), sliding_attention(*batch, 1 << 30))
+
+
+@pytest.mark.parametrize("rows", [[1] * 5, [40, 1, 300]])
+def test_strides_of_q_and_out(rows):
+    """q as a view of a projection's rows, out as a view of a wider buffer, and out in the place of q: the same bits."""
+    from monoserve_b200.attention import sliding_attention
+    past = [100 * (r + 1) for r in range(len(rows))]
+    q, kc, vc, bt, start, kv = on_gpu(*make(rows, past, 32, 4, 128, 16, BF, seed=13))
+    want = sliding_attention(q, kc, vc, bt, start, kv, 150, sinks=2)
+    qkv = torch.zeros(len(q), 40, 128, dtype=BF, device="cuda")
+    qkv[:, :32] = q
+    wide = torch.full((len(q), 33, 160), 3.0, dtype=BF, device="cuda")
+    sliding_attention(qkv[:, :32], kc, vc, bt, start, kv, 150, sinks=2, out=wide[:, :32, 8:136])
+    assert torch.equal(wide[:, :32, 8:136], want)
+    assert bool((wide[:, 32] == 3).all()) and bool((wide[:, :, :8] == 3).all()) and bool((wide[:, :, 136:] == 3).all())
+    sliding_attention(qkv[:, :32], kc, vc, bt, start, kv, 150, sinks=2, out=qkv[:, :32])
+    assert torch.equal(qkv[:, :32], want) and bool((qkv[:, 32:] == 0).all())
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(sliding_attention(heads_first, kc, vc, bt, start, kv, 150, sinks=2), want)
+
+
+def test_the_same_bits_every_time():
+    from monoserve_b200.attention import sliding_attention
+    batch = on_gpu(*make([1, 1, 200, 1], [9000, 3000, 500, 20], 32, 4, 128, 16, BF, seed=14))
+    want = sliding_attention(*batch, 1 << 30)
+    assert all(torch.equal(sliding_attention(*batch, 1 << 30), want) for _ in range(20))
+
+
+def test_a_captured_call_takes_the_lengths_of_its_replay():
+    from monoserve_b200.attention import sliding_attention
+    long = make([1, 1, 1], [700, 2000, 5000], 32, 4, 128, 16, BF, seed=15)
+    q, kc, vc, bt, start, kv = on_gpu(*long)
+    sliding_attention(q, kc, vc, bt, start, kv, 900, sinks=4)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = sliding_attention(q, kc, vc, bt, start, kv, 900, sinks=4)
+    for lens in ([701, 2001, 5001], [3, 1500, 1], [701, 0, 4999]):
+        kv.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        batch = (*long[:5], torch.tensor(lens, dtype=torch.int32))
+        check(out, batch, [sliding_mask(1, L, 900, 4) if L else torch.zeros(1, 0, dtype=torch.bool) for L in lens])
+
+
+def test_calls_on_two_streams_and_two_graphs_at_once():
+    """Calls that overlap do not share a workspace."""
+    from monoserve_b200.attention import sliding_attention
+    batches = [on_gpu(*make([1, 1], [6000 + s, 3000], 32, 4, 128, 16, BF, seed=16 + s)) for s in range(2)]
+    want = [sliding_attention(*b, 1 << 30) for b in batches]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[sliding_attention(*b, 1 << 30, stream=st) for _ in range(8)] for b, st in zip(batches, streams)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for outs, w in zip(got, want) for o in outs)
+    graphs, outs = [], []
+    for b in batches:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(sliding_attention(*b, 1 << 30))
+        graphs.append(g)
+    for _ in range(5):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_a_cache_past_32_bits():
+    """Pages whose first value lies past 2^31 values."""
+    from monoserve_b200.attention import sliding_attention
+    batch = make([1, 20], [200, 100], 8, 8, 128, 64, BF, seed=18, extra_pages=1)
+    q, kc, vc, bt, start, kv = batch
+    n = kc.shape[0]
+    far = (1 << 31) // kc[0].numel() + 3
+    big = [torch.empty(far + n, *kc.shape[1:], dtype=BF, device="cuda") for _ in range(2)]
+    for b, c in zip(big, (kc, vc)):
+        b[far:] = c.cuda()
+    out = sliding_attention(q.cuda(), *big, (bt + far).cuda(), start.cuda(), kv.cuda(), 150)
+    check(out, batch, sliding_masks(batch, 150, 0))
+
+
+def test_many_requests_most_of_them_empty():
+    rows = [1 if r % 37 == 0 else 0 for r in range(1500)]
+    past = [r % 400 for r in range(1500)]
+    batch = make(rows, past, 4, 2, 64, 16, FP, seed=19)
+    check(run_sliding(batch, 100, 1), batch, sliding_masks(batch, 100, 1))
+
+
+def test_scale_and_large_scores():
+    """Weights that are all but zero and maxima that grow from tile to tile."""
+    q, kc, vc, bt, start, kv = make([1, 70], [1000, 500], 8, 2, 128, 16, BF, seed=20)
+    batch = (q, kc, vc, bt, start, kv)
+    check(run_sliding(batch, 1 << 30, 0, scale=1e-4), batch, sliding_masks(batch, 1 << 30, 0), scale=1e-4)
+    ramp = torch.arange(kc.shape[0] * 16).view(-1, 16, 1, 1) / 1024
+    batch = (q.sign(), (kc.sign() * ramp).to(BF), vc, bt, start, kv)
+    out = run_sliding(batch, 1 << 30, 0, scale=1.0)
+    ref, weighted = reference(*batch, sliding_masks(batch, 1 << 30, 0), scale=1.0)
+    # 128 exact products below 1.8: their 32-bit sum is off by less than 128 * 2^-24 * 128 * 1.8 = 1.8e-3
+    tol = tolerance(ref, weighted, BF, 1100) + 1.8e-3 * weighted
+    err = (out.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())

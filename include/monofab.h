@@ -140,8 +140,8 @@ int monofab_attention(const void* q, const void* k_cache, const void* v_cache, v
  *   else           the past (j < kv_len - rows) and the drafted tokens whose bit is set: of drafted token d bit d % 32 of
  *                  tree[row][d / 32]; those from 32 * words on have none.
  * out = sum_j softmax_j(scale q k_j) v_j; a row that sees no key is zeros.  Rows of no request keep what they hold.
- * Values of keys that a request's row sees must be finite, also for that request's rows that do not see them; what no row
- * of a request sees may hold anything.
+ * Keys and values of drafted tokens, and of what any row of a request sees, must be finite, also for that request's rows that
+ * do not see them; what no row of a request sees may hold anything.  At most 16384 requests a call.
  * Keys past the block table (kv_len > bt_stride * page_size) are not there; a page number outside [0, n_pages) reads as
  * zeros; q_start is taken as ascending within [0, tokens], and a request that it gives no rows has none. */
 typedef struct {
@@ -153,7 +153,7 @@ typedef struct {
   const int32_t* q_start;      /* [requests + 1] */
   const int32_t* kv_len;       /* [requests] */
   const int32_t* tree;         /* [tokens][words], or NULL */
-  void* ws;                    /* monofab_masked_attention_ws_bytes(...) bytes that the call may overwrite; calls whose kernels
+  void* ws;                    /* monofab_masked_attention_ws_bytes(head_dim) bytes that the call may overwrite; calls whose kernels
                                   overlap on the GPU need one each */
   int32_t* status;             /* receives MONOFAB_STATUS_WAIT_TIMEOUT if a bounded wait ran out; NULL: the device's own word */
   int64_t q_row, q_head, out_row, out_head, ws_bytes;
@@ -163,7 +163,8 @@ typedef struct {
   float scale;                 /* of the scores, positive */
   int32_t reserved;
 } monofab_masked_attention_args;
-size_t monofab_masked_attention_ws_bytes(int tokens, int hq, int hkv, int head_dim);
+/* Bytes of a call's workspace on the current device, or a negative error code. */
+int64_t monofab_masked_attention_ws_bytes(int head_dim);
 int monofab_masked_attention(const monofab_masked_attention_args* args, void* stream);
 /* The current device's own status word of these calls, read (the device is synchronised) and cleared. */
 int monofab_masked_attention_status(int32_t* out);

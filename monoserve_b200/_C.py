@@ -82,8 +82,8 @@ def _load():
     lib.monofab_attention.argtypes = [vp, vp, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, i32, vp, i32, vp, vp]
     lib.monofab_attention_trace.argtypes = [i32, vp]
     i64 = ctypes.c_int64
-    lib.monofab_masked_attention_ws_bytes.restype = ctypes.c_size_t
-    lib.monofab_masked_attention_ws_bytes.argtypes = [i32, i32, i32, i32]
+    lib.monofab_masked_attention_ws_bytes.restype = i64
+    lib.monofab_masked_attention_ws_bytes.argtypes = [i32]
     lib.monofab_masked_attention.argtypes = [ctypes.POINTER(MaskedAttentionArgsC), vp]
     lib.monofab_masked_attention_status.argtypes = [ctypes.POINTER(ctypes.c_int32)]
     lib.monofab_qk_rope.argtypes = [vp, i64, vp, vp, vp, i32, vp, vp, vp, i64, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, f32, vp]

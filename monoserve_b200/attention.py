@@ -175,8 +175,12 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     _refuse(0.0 < scale < math.inf, "the scale must be positive and finite")
     if out is not None:
         _refuse(out.shape == q.shape and out.dtype == q.dtype, "out has the shape and type of q")
+    def strides(t):   # of rows and heads; of a single one it may be anything
+        return t.stride(0) if T > 1 else hq * D, t.stride(1) if hq > 1 else D
+
     for t in (q,) if out is None else (q, out):
-        _refuse(T == 0 or (t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.stride(0) >= 0 and t.stride(1) > 0 and t.data_ptr() % 16 == 0),
+        (q_row, q_head), last = strides(t), t.stride(2)
+        _refuse(T == 0 or (last == 1 and q_row % 8 == 0 and q_head % 8 == 0 and q_row > 0 and q_head > 0 and t.data_ptr() % 16 == 0),
                 "the heads of q and out must be contiguous and start at multiples of 16 bytes")
     device = q.device
     _refuse(q.is_cuda and all(t.device == device for t in (k_cache, v_cache, *small)) and (out is None or out.device == device) and
@@ -189,12 +193,14 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
                 out = torch.empty((T, hq, D), dtype=q.dtype, device=device)
             if T == 0 or R == 0:
                 return out
-            ws_bytes = _C.lib.monofab_masked_attention_ws_bytes(T, hq, hkv, D)
+            ws_bytes = _C.lib.monofab_masked_attention_ws_bytes(D)
+            if ws_bytes < 0:
+                _C.check(ws_bytes)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
         a = _C.MaskedAttentionArgsC(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
             None if tree is None else tree.data_ptr(), ws.data_ptr(), None if status is None else status.data_ptr(),
-            q.stride(0), q.stride(1), out.stride(0), out.stride(1), ws_bytes, T, R, hq, hkv, D, page, n_pages, block_table.shape[1], words,
+            *strides(q), *strides(out), ws_bytes, T, R, hq, hkv, D, page, n_pages, block_table.shape[1], words,
             0 if tree is not None else window, 0 if tree is not None else sinks, int(q.dtype == torch.float16), scale, 0)
         _C.check(_C.lib.monofab_masked_attention(ctypes.byref(a), ctypes.c_void_p(st.cuda_stream)))
     return out
@@ -210,7 +216,7 @@ def sliding_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     on the device: a call captured in a CUDA graph can be replayed with others.  Returns [T, hq, D] (`out`, which may be q
     itself): rows that see no key are zeros, rows of no request keep what they hold (are undefined in a new tensor).
     A bounded wait that ran out is reported in `status` (int32 on the device), or to attention_status().  Keys that some row of
-    a request sees must hold finite values; the others may hold anything."""
+    a request sees must hold finite values; the others may hold anything.  At most 16384 requests."""
     return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, int(window), int(sinks), None, scale, out, stream, status)
 
 

@@ -1,99 +1,957 @@
-// Attention over a paged cache with a window and sinks, or with a tree of drafted tokens behind the past.
+// Attention over a paged cache with a window and sinks, or with a tree of drafted tokens behind the past, on tcgen05 /
+// TMEM / TMA.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
+#include "kernels.h"
 #include "masked_attention.h"
 #include "moe_layer.h"
+#include "ptx.cuh"
 
 namespace mf {
 
+int encode_map(CUtensorMap* map, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+               int swizzle);   // api.cu
+
 namespace {
 
-template <class E>
-__device__ __forceinline__ float to_float(E x) {
-  return static_cast<float>(x);
-}
-
-// A warp per (row, query head), keys one after the other.
-template <class E, int D>
-__global__ void __launch_bounds__(256) masked_attention_kernel(const __grid_constant__ MaskedAttnParams p) {
-  chain_release();
-  chain_wait();
-  const int lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * 8 + threadIdx.x / 32;
-  const int head = static_cast<int>(item % p.hq);
-  const long long row = item / p.hq;
-  if (row >= p.tokens) return;
-  int lo = 0, hi = p.requests;   // the last request that starts at or before the row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (p.q_start[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  const int first = p.q_start[lo], end = p.q_start[lo + 1];
-  if (row < first || row >= end) return;
-  const int n = end - first, i = static_cast<int>(row) - first;
-  const int keys = min(p.kv_len[lo], p.bt_stride * p.page_size), past = p.kv_len[lo] - n, pos = past + i;
-  const E* const q = static_cast<const E*>(p.q) + row * p.q_row + head * p.q_head;
-  const int kvh = head / (p.hq / p.hkv);
-  constexpr int N = D / 32;
-  float qv[N], o[N], m = -INFINITY, l = 0.f;
-  for (int d = 0; d < N; ++d) qv[d] = to_float(q[lane + 32 * d]) * p.scale, o[d] = 0.f;
-  for (int key = 0; key < keys; ++key) {
-    bool seen;
-    if (p.tree) {
-      const int j = key - past;
-      seen = j < 0 || (j < 32 * p.words && j < n && (p.tree[row * p.words + j / 32] >> (j % 32) & 1));
-    } else {
-      seen = key <= pos && (key > pos - static_cast<long long>(p.window) || key < p.sinks);
-    }
-    if (!seen) continue;
-    const long long at = ((static_cast<long long>(p.block_table[static_cast<long long>(lo) * p.bt_stride + key / p.page_size]) * p.page_size + key % p.page_size) * p.hkv + kvh) * D;
-    const E *const k = static_cast<const E*>(p.k_cache) + at, *const v = static_cast<const E*>(p.v_cache) + at;
-    float s = 0.f;
-    for (int d = 0; d < N; ++d) s += qv[d] * to_float(k[lane + 32 * d]);
-    for (int bit = 16; bit; bit >>= 1) s += __shfl_xor_sync(0xffffffffu, s, bit);
-    const float top = fmaxf(m, s), keep = expf(m - top), w = expf(s - top);
-    m = top;
-    l = l * keep + w;
-    for (int d = 0; d < N; ++d) o[d] = o[d] * keep + w * to_float(v[lane + 32 * d]);
-  }
-  E* const out = static_cast<E*>(p.out) + row * p.out_row + head * p.out_head;
-  for (int d = 0; d < N; ++d) out[lane + 32 * d] = static_cast<E>(l > 0.f ? o[d] / l : 0.f);
-}
+constexpr int kTile = 128;          // keys of a tile, rows of a stream
+constexpr int kThreads = 384;
+constexpr int kRecords = 4;
+constexpr int kItemCost = 2;        // what an item costs beyond its tiles, in tiles
+constexpr int kMinCost = 4;         // of a CTA's share
+constexpr int kSlotRows = 2 * kTile;
+constexpr int kMaxRequests = 16384;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr float kSlack = 8.f;
 
 // Where a call that names no status word leaves its bits.
 __device__ int g_masked_attention_status;
 
-}  // namespace
+struct Params {
+  CUtensorMap q_map;      // dims (D, hq, tokens), box (64, group, tokens of a stream)
+  CUtensorMap q_one_map;  // box (64, group, 1)
+  CUtensorMap k_map;      // dims (64, 8, halves x hkv, page / 8, pages), box (64, 8, halves, page / 8, 1)
+  CUtensorMap v_map;
+  const int32_t *block_table, *q_start, *kv_len, *tree;
+  void* out;
+  int* status;
+  float* ws_o;            // [2 x CTAs][256][D]
+  float2* ws_ml;          // [2 x CTAs][256]
+  int4* ws_meta;          // [CTAs][2]
+  long long out_row, out_head;
+  int tokens, requests, hkv, group, page, n_pages, bt_stride, words, window, sinks;
+  int per_stream;         // query tokens of a stream's 128 rows
+  float scale_log2;
+};
 
-cudaError_t launch_masked_attention(const MaskedAttnParams& p, cudaStream_t stream) {
-  auto go = [&](auto kernel) {
-    return launch_chained(kernel, dim3(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.hq + 7) / 8)), dim3(256), 0, stream, p);
-  };
-  if (p.fp16) return p.head_dim == 64 ? go(masked_attention_kernel<__half, 64>) : go(masked_attention_kernel<__half, 128>);
-  return p.head_dim == 64 ? go(masked_attention_kernel<__nv_bfloat16, 64>) : go(masked_attention_kernel<__nv_bfloat16, 128>);
+// A request as the device sees it.
+struct Request {
+  int row0, rows, kv_len;
+};
+__device__ __forceinline__ Request request_of(const Params& p, int r) {
+  Request q;
+  q.row0 = max(0, min(p.q_start[r], p.tokens));
+  q.rows = max(0, min(p.q_start[r + 1], p.tokens) - q.row0);
+  q.kv_len = max(0, p.kv_len[r]);
+  return q;
 }
+__device__ __forceinline__ int blocks_of(const Params& p, int rows) { return (rows + 2 * p.per_stream - 1) / (2 * p.per_stream); }
+
+// The keys that the rows of a block see lie in [0, near) and [lo, hi); they are covered by sink_tiles tiles from 0 on and by
+// win_tiles from tile win_tile0 on.
+struct Span {
+  int tokens, pos0, lo, hi, near, sink_tiles, win_tile0, win_tiles;
+  __device__ __forceinline__ int tiles() const { return sink_tiles + win_tiles; }
+};
+__device__ __forceinline__ Span span_of(const Params& p, const Request& q, int block) {
+  Span s;
+  const int first = block * 2 * p.per_stream;
+  s.tokens = min(2 * p.per_stream, q.rows - first);
+  s.pos0 = q.kv_len - q.rows + first;
+  const int there = min(q.kv_len, p.bt_stride * p.page);
+  if (p.tree) {
+    s.lo = s.near = 0;
+    s.hi = there;
+  } else {
+    s.hi = max(0, min(there, s.pos0 + s.tokens));
+    s.lo = static_cast<int>(max(0ll, static_cast<long long>(s.pos0) - p.window + 1));
+    s.near = min(min(p.sinks, s.hi), s.lo);
+  }
+  s.win_tile0 = s.lo / kTile;
+  s.win_tiles = max(0, (s.hi + kTile - 1) / kTile - s.win_tile0);
+  s.sink_tiles = min((s.near + kTile - 1) / kTile, s.win_tile0);
+  return s;
+}
+
+// A CTA's share of the work begins at tile t of (request, block, head); r == requests: the end.
+struct Place {
+  int r, b, h, t;
+};
+__device__ __forceinline__ bool same_item(const Place& a, const Place& b) { return a.r == b.r && a.b == b.b && a.h == b.h; }
+
+// One part of an item, as the roles get it.
+struct Record {
+  int req, head, row0, tokens, pos0, past, there;   // there: keys in the block table; past: first drafted key
+  int lo, hi, near;
+  int sink_tiles, win_tile0, t0, t1;
+  int slot;     // -1: the whole item, else the workspace slot
+  int pair;     // two streams of rows; else the streams take alternate tiles. -1: no more items
+  __device__ __forceinline__ int tile_key(int t) const { return kTile * (t < sink_tiles ? t : t - sink_tiles + win_tile0); }
+};
+
+template <int D>
+struct Layout {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kGroupBytes = 1024 * kHalves;   // eight keys of a K or V tile
+  static constexpr int kSmem = (2 + kStages) * kTileBytes;
+};
+
+struct Shared {
+  uint64_t kv_full[10], kv_empty[10], rec_full[kRecords], rec_empty[kRecords];
+  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], x_full, x_done, drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  Place place[2];
+  Record rec[kRecords];
+  float2 ml[2][kTile];
+};
+
+// Descriptors: Q rows of 128 bytes a half, halves 16 KB apart; K and V tiles in groups of eight keys, the halves of a group
+// 1 KB apart (one TMA box of a page delivers both).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 | static_cast<uint64_t>(stride >> 4) << 32 |
+         static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]; issued by one thread.
+__device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void load_box_3d(void* smem, const void* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               :
+               : "r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void load_box_5d(void* smem, const void* map, uint64_t* bar, int c2, int c4) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %4, %3, %5}], [%2];"
+               :
+               : "r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(c2), "r"(c4)
+               : "memory");
+}
+__device__ __forceinline__ void store_tmem_32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void store_tmem_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <class E>
+struct Half2;
+template <>
+struct Half2<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = 1;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Half2<__half> {
+  static constexpr uint32_t kFormat = 0;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <class E>
+__host__ __device__ constexpr uint32_t idesc_of(int n) {   // fp32 accumulators, M = 128
+  return (1u << 4) | (Half2<E>::kFormat << 7) | (Half2<E>::kFormat << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+// Bits of [lo, hi) in a word.
+__device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
+  lo = max(lo, 0), hi = min(hi, 32);
+  if (lo >= hi) return 0u;
+  return (0xffffffffu >> (32 - (hi - lo))) << lo;
+}
+
+// ---------------------------------------------------------------------------------------------------- the shares
+
+// Tiles and items of a request as cost, by `lanes` neighbouring lanes.
+__device__ __forceinline__ long long request_cost(const Params& p, const Request& q, int lane, int lanes) {
+  long long sum = 0;
+  const int n = blocks_of(p, q.rows);
+  for (int b = lane; b < n; b += lanes) sum += span_of(p, q, b).tiles() + kItemCost;
+  for (int bit = lanes / 2; bit >= 1; bit >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
+  return sum * p.hkv;
+}
+
+// Place number k of `shares` equal parts of the total cost, by a warp. prefix: inclusive sums over the requests. A place within a
+// sixteenth of a share from an item's begin is put there.
+__device__ Place place_of(const Params& p, const long long* prefix, long long total, int shares, int k) {
+  const int lane = threadIdx.x & 31;
+  Place at{p.requests, 0, 0, 0};
+  if (k >= shares) return at;
+  const long long target = total * k / shares;
+  int lo = 0, hi = p.requests - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (prefix[mid] > target) hi = mid;
+    else lo = mid + 1;
+  }
+  at.r = lo;
+  const Request q = request_of(p, lo);
+  long long rest = target - (lo ? prefix[lo - 1] : 0);
+  const int blocks = blocks_of(p, q.rows);
+  int cost = 0;
+  for (int b0 = 0; b0 < blocks; b0 += 32) {   // 32 blocks at a time
+    const int mine = b0 + lane < blocks ? span_of(p, q, b0 + lane).tiles() + kItemCost : 0;
+    long long sum = static_cast<long long>(mine) * p.hkv;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, sum > rest);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      cost = __shfl_sync(0xffffffffu, mine, l);
+      rest -= __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(cost) * p.hkv;
+      at.b = b0 + l;
+      break;
+    }
+    rest -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  at.h = static_cast<int>(rest / cost);
+  const int off = static_cast<int>(rest - static_cast<long long>(at.h) * cost);
+  const long long near = total / shares / 16;
+  if (off <= kItemCost || off <= near) return at;
+  if (cost - off > near) {
+    at.t = off - kItemCost;
+    return at;
+  }
+  if (++at.h == p.hkv) {
+    at.h = 0;
+    if (++at.b == blocks) {
+      at.b = 0;
+      do ++at.r;
+      while (at.r < p.requests && prefix[at.r] == prefix[at.r - 1]);
+    }
+  }
+  return at;
+}
+
+// Writes the records of the items from place[0] to place[1].
+__device__ void schedule(const Params& p, Shared& sh) {
+  const int lane = threadIdx.x & 31;
+  Place at = sh.place[0];
+  const Place end = sh.place[1];
+  int seen_from = -1;
+  Request seen{0, 0, 0};
+  for (int n = 0;; ++n) {
+    Record rec;
+    rec.pair = -1;
+    if (at.r < p.requests && !(same_item(at, end) && end.t <= at.t)) {
+      if (seen_from < 0 || at.r >= seen_from + 32) {   // 32 requests in the lanes
+        seen_from = at.r;
+        if (at.r + lane < p.requests) seen = request_of(p, at.r + lane);
+      }
+      Request q;
+      const int from = at.r - seen_from;
+      q.row0 = __shfl_sync(0xffffffffu, seen.row0, from);
+      q.rows = __shfl_sync(0xffffffffu, seen.rows, from);
+      q.kv_len = __shfl_sync(0xffffffffu, seen.kv_len, from);
+      const int blocks = blocks_of(p, q.rows);
+      if (at.b >= blocks) {   // a request without rows, or the end of one
+        ++at.r;
+        at.b = 0;
+        --n;
+        continue;
+      }
+      const Span s = span_of(p, q, at.b);
+      const int tiles = s.tiles();
+      rec.req = at.r;
+      rec.head = at.h;
+      rec.row0 = q.row0 + at.b * 2 * p.per_stream;
+      rec.tokens = s.tokens;
+      rec.pos0 = s.pos0;
+      rec.past = q.kv_len - q.rows;
+      rec.there = min(q.kv_len, p.bt_stride * p.page);
+      rec.lo = s.lo;
+      rec.hi = s.hi;
+      rec.near = s.near;
+      rec.sink_tiles = s.sink_tiles;
+      rec.win_tile0 = s.win_tile0;
+      rec.t0 = at.t;
+      rec.t1 = same_item(at, end) ? end.t : tiles;
+      const int cta = static_cast<int>(blockIdx.x);
+      rec.slot = rec.t0 > 0 ? 2 * cta : rec.t1 < tiles ? 2 * cta + 1 : -1;
+      rec.pair = s.tokens > p.per_stream;
+      at.t = 0;
+      if (same_item(at, end)) at.r = p.requests;   // nothing behind it
+      else if (++at.h == p.hkv) {
+        at.h = 0;
+        ++at.b;
+      }
+    }
+    const int slot = n % kRecords;
+    if (n >= kRecords && !mbar_wait_warp(&sh.rec_empty[slot], (n / kRecords - 1) & 1, &sh.abort_flag, kWaitNs)) return;
+    if (lane == 0) {
+      sh.rec[slot] = rec;
+      mbar_arrive(&sh.rec_full[slot]);
+    }
+    __syncwarp();
+    if (rec.pair < 0) return;
+  }
+}
+
+// The next record, by every warp of a role alike. False: no more.
+struct Records {
+  int n = 0;
+  __device__ __forceinline__ bool next(Shared& sh, Record& rec) {
+    const int slot = n % kRecords;
+    if (!mbar_wait_warp(&sh.rec_full[slot], (n / kRecords) & 1, &sh.abort_flag, kWaitNs)) return false;
+    rec = sh.rec[slot];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.rec_empty[slot]);
+    ++n;
+    return rec.pair >= 0;
+  }
+};
+
+// Stage of the operand ring and its parity.
+template <int kStages>
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// Whether any row of the item sees key `key`.
+__device__ __forceinline__ bool some_row_sees(const Record& rec, int key) { return key < rec.hi && (key >= rec.lo || key < rec.near); }
+
+// ------------------------------------------------------------------------------------------------------ the roles
+
+template <int D>
+__device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
+  using L = Layout<D>;
+  const int lane = threadIdx.x & 31;
+  const int pages = kTile / p.page, page_bytes = p.page * D * 2;
+  Ring<L::kStages> ring;
+  uint32_t loads = 0;
+  Records records;
+  Record rec;
+  auto run = [&] {
+  while (records.next(sh, rec)) {
+    const int n = rec.t1 - rec.t0, lead = rec.pair ? 0 : 1;   // K runs one tile ahead of V where the streams take alternate tiles
+    const int32_t* const table = p.block_table + static_cast<size_t>(rec.req) * p.bt_stride;
+    int ahead = 0;   // this lane's page of the tile of `step`, and whether some row sees a key of it
+    bool there = false;
+    auto look_up = [&](int j) {
+      const int key = rec.tile_key(rec.t0 + j) + lane * p.page;
+      there = lane < pages && key < rec.hi && (key + p.page > rec.lo || key < rec.near);
+      ahead = there ? table[key / p.page] : 0;
+    };
+    int last_page = 0;
+    bool last_there = false;
+    auto load = [&](const CUtensorMap* map, int page, bool wanted) {
+      if (!mbar_wait_warp(&sh.kv_empty[ring.stage], ring.phase ^ 1, &sh.abort_flag, kWaitNs)) return false;
+      const uint32_t which = __ballot_sync(0xffffffffu, wanted);
+      if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[ring.stage], __popc(which) * page_bytes);
+      __syncwarp();
+      if (wanted) load_box_5d(ring_mem + ring.stage * L::kTileBytes + lane * page_bytes, map, &sh.kv_full[ring.stage], L::kHalves * rec.head, page);
+      ring.advance();
+      ++loads;
+      return true;
+    };
+    for (int step = 0; step < n + lead; ++step) {
+      if (step < n) {
+        look_up(step);
+        if (!load(&p.k_map, ahead, there)) return;
+      }
+      if (lead == 0) {
+        if (!load(&p.v_map, ahead, there)) return;
+      } else {
+        if (step > 0 && !load(&p.v_map, last_page, last_there)) return;
+        last_page = ahead;
+        last_there = there;
+      }
+    }
+  }
+  };
+  run();
+  // however it ended, the last loads have landed before the CTA's memory is given up
+  for (uint32_t i = loads > L::kStages ? loads - L::kStages : 0; i < loads; ++i) {
+    int ignored = 0;
+    mbar_wait_warp(&sh.kv_full[i % L::kStages], (i / L::kStages) & 1, &ignored, kWaitNs);
+  }
+}
+
+template <int D>
+__device__ void load_queries(const Params& p, Shared& sh, uint8_t* q_mem) {
+  using L = Layout<D>;
+  const int lane = threadIdx.x & 31;
+  Records records;
+  Record rec;
+  int uses = 0;
+  while (records.next(sh, rec)) {
+    if (rec.t0 == rec.t1) continue;
+    if (uses > 0 && !mbar_wait_warp(&sh.q_empty, (uses - 1) & 1, &sh.abort_flag, kWaitNs)) break;
+    ++uses;
+    if (lane == 0) {
+      const bool one = rec.tokens == 1;
+      const CUtensorMap* const map = one ? &p.q_one_map : &p.q_map;
+      const int rows = p.group * (one ? 1 : p.per_stream);
+      mbar_arrive_expect_tx(&sh.q_full, (1 + rec.pair) * L::kHalves * rows * 128);
+      for (int s = 0; s <= rec.pair; ++s)
+        for (int h = 0; h < L::kHalves; ++h)
+          load_box_3d(q_mem + s * L::kTileBytes + h * (kTile * 128), map, &sh.q_full, 64 * h, rec.head * p.group, rec.row0 + s * p.per_stream);
+    }
+    __syncwarp();
+  }
+  int ignored = 0;
+  if (uses > 0) mbar_wait_warp(&sh.q_full, (uses - 1) & 1, &ignored, kWaitNs);
+}
+
+template <class E, int D>
+__device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* ring_mem) {
+  using L = Layout<D>;
+  const int lane = threadIdx.x & 31;
+  const bool leader = elect_one();
+  const uint32_t tmem = sh.tmem_base;
+  constexpr uint32_t idesc_s = idesc_of<E>(kTile), idesc_o = idesc_of<E>(D) | (1u << 16);   // V is MN-major
+  Ring<L::kStages> ring;
+  Records records;
+  Record rec{};
+  int q_uses = 0;
+  uint32_t p_count[2] = {0, 0};
+  auto wait_stage = [&] { return mbar_wait_warp(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag, kWaitNs); };
+  auto scores = [&](int x, int q_tile, int stage) {   // S[x] = Q K^T
+    if (!leader) return;
+    const uint32_t q = smem_u32(q_mem) + q_tile * L::kTileBytes, k = smem_u32(ring_mem) + stage * L::kTileBytes;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      umma_bf16(tmem + x * 128, smem_desc(q + (i >> 2) * (kTile * 128) + (i & 3) * 32, 0, 1024),
+                smem_desc(k + (i >> 2) * 1024 + (i & 3) * 32, 0, L::kGroupBytes), idesc_s, i != 0);
+    umma_commit(&sh.s_full[x]);
+  };
+  auto values = [&](int x, int stage, bool accumulate) {   // O[x] (+)= P[x] V
+    if (!leader) return;
+    const uint32_t v = smem_u32(ring_mem) + stage * L::kTileBytes;
+#pragma unroll
+    for (int i = 0; i < kTile / 16; ++i)
+      umma_tmem_a(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, smem_desc(v + i * 2 * L::kGroupBytes, 1024, L::kGroupBytes), idesc_o,
+                  accumulate || i != 0);
+  };
+  auto wait_weights = [&](int x) {
+    const bool ok = mbar_wait_warp(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag, kWaitNs);
+    ++p_count[x];
+    tc_fence_after_sync();
+    return ok;
+  };
+  // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none.
+  auto clean = [&](int stage, int key0) {
+    if (key0 + kTile <= rec.hi && (key0 >= rec.lo || key0 + kTile <= rec.near)) return;
+    uint8_t* const v = ring_mem + stage * L::kTileBytes;
+    for (int i = lane / 8; i < kTile * L::kHalves; i += 4) {
+      const int k = i / L::kHalves;
+      if (!some_row_sees(rec, key0 + k))
+        *reinterpret_cast<uint4*>(v + (k >> 3) * L::kGroupBytes + (i % L::kHalves) * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+  };
+  auto run = [&] {
+    while (records.next(sh, rec)) {
+      const int n = rec.t1 - rec.t0;
+      if (n == 0) continue;
+      if (!mbar_wait_warp(&sh.q_full, q_uses & 1, &sh.abort_flag, kWaitNs)) return;
+      ++q_uses;
+      if (!wait_stage()) return;
+      tc_fence_after_sync();
+      scores(0, 0, ring.stage);
+      if (rec.pair) {
+        scores(1, 1, ring.stage);
+        if (leader) umma_commit(&sh.kv_empty[ring.stage]);
+        if (leader && n == 1) umma_commit(&sh.q_empty);
+        ring.advance();
+        for (int j = 0; j < n; ++j) {
+          if (!wait_stage()) return;
+          const int v_stage = ring.stage;
+          clean(v_stage, rec.tile_key(rec.t0 + j));
+          ring.advance();
+          if (!wait_weights(0)) return;
+          values(0, v_stage, j > 0);
+          if (j + 1 < n) {
+            if (!wait_stage()) return;
+            tc_fence_after_sync();
+            scores(0, 0, ring.stage);
+          } else if (leader) {
+            umma_commit(&sh.o_full[0]);
+          }
+          if (!wait_weights(1)) return;
+          values(1, v_stage, j > 0);
+          if (leader) umma_commit(&sh.kv_empty[v_stage]);
+          if (j + 1 < n) {
+            scores(1, 1, ring.stage);
+            if (leader) umma_commit(&sh.kv_empty[ring.stage]);
+            if (leader && j + 2 == n) umma_commit(&sh.q_empty);
+            ring.advance();
+          } else if (leader) {
+            umma_commit(&sh.o_full[1]);
+          }
+        }
+        continue;
+      }
+      if (leader) umma_commit(&sh.kv_empty[ring.stage]);
+      ring.advance();
+      if (n > 1) {
+        if (!wait_stage()) return;
+        tc_fence_after_sync();
+        scores(1, 0, ring.stage);
+        if (leader) umma_commit(&sh.kv_empty[ring.stage]);
+        ring.advance();
+      }
+      if (leader && n <= 2) umma_commit(&sh.q_empty);
+      for (int j = 0; j < n; ++j) {
+        const int x = j & 1;
+        if (!wait_stage()) return;
+        clean(ring.stage, rec.tile_key(rec.t0 + j));
+        if (!wait_weights(x)) return;
+        values(x, ring.stage, j > 1);
+        if (leader) umma_commit(&sh.kv_empty[ring.stage]);
+        ring.advance();
+        if (j + 2 < n) {
+          if (!wait_stage()) return;
+          tc_fence_after_sync();
+          scores(x, 0, ring.stage);
+          if (leader) umma_commit(&sh.kv_empty[ring.stage]);
+          if (leader && j + 3 == n) umma_commit(&sh.q_empty);
+          ring.advance();
+        }
+      }
+      if (leader) umma_commit(&sh.o_full[0]);
+      if (leader) umma_commit(&sh.o_full[1]);
+    }
+  };
+  run();
+  // whatever ended the loop: nothing of this warp is in flight when it leaves
+  if (leader) umma_commit(&sh.drain);
+  int ignored = 0;
+  mbar_wait_warp(&sh.drain, 0, &ignored, kWaitNs);
+}
+
+template <class E, int D>
+__device__ void softmax(const Params& p, Shared& sh, int wg) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, r = quad * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+  const uint32_t tmem_s = sh.tmem_base + wg * 128 + lanes, tmem_o = sh.tmem_base + 256 + lanes;
+  const int token_in = r / p.group, head_in = r - token_in * p.group;
+  uint32_t s_count = 0, o_count = 0, x_count = 0;
+  Records records;
+  Record rec;
+  const float scale = p.scale_log2;
+  while (records.next(sh, rec)) {
+    const int n = rec.t1 - rec.t0;
+    const int first = rec.pair ? wg * p.per_stream : 0;                       // first token of the stream in the item
+    const int tokens = min(rec.tokens - first, p.per_stream);
+    const bool row_ok = r < tokens * p.group;
+    const bool works = quad * 32 < tokens * p.group;                           // warp-uniform
+    const int token = first + token_in, row = rec.row0 + token, head = rec.head * p.group + head_in;
+    const int pos = rec.pos0 + token;
+    const int pos_first = rec.pos0 + first, pos_last = pos_first + tokens - 1;
+    float m = -INFINITY, l = 0.f;
+    bool begun = false;
+    for (int j = rec.pair ? 0 : wg; j < n; j += rec.pair ? 1 : 2) {
+      if (!mbar_wait_warp(&sh.s_full[wg], s_count & 1, &sh.abort_flag, kWaitNs)) return;
+      ++s_count;
+      tc_fence_after_sync();
+      if (!works) {   // no row of this warp exists
+        tc_fence_before_sync();
+        mbar_arrive(&sh.p_full[wg]);
+        continue;
+      }
+      const int key0 = rec.tile_key(rec.t0 + j);
+      uint32_t v[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(tmem_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+      tmem_ld_wait();
+      bool full;
+      if (p.tree) full = key0 + kTile <= min(rec.past, rec.there);
+      else
+        full = key0 + kTile - 1 <= pos_first && key0 + kTile <= rec.there &&
+               (static_cast<long long>(key0) > static_cast<long long>(pos_last) - p.window || key0 + kTile <= p.sinks);
+      if (!full) {
+        // what the row sees of the tile, as 128 bits
+        uint32_t seen[4];
+        if (p.tree) {
+          const int32_t* const words = p.tree + static_cast<size_t>(row_ok ? row : rec.row0) * p.words;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int d = key0 + 32 * c - rec.past;   // the drafted token of the first column
+            const int w = d >> 5, s = d & 31;         // floor
+            const uint32_t a = w >= 0 && w < p.words ? words[w] : 0u, b = w + 1 >= 0 && w + 1 < p.words ? words[w + 1] : 0u;
+            seen[c] = (__funnelshift_r(a, b, s) | bits_of(0, -d)) & bits_of(0, rec.there - key0 - 32 * c);
+          }
+        } else {
+          const int hi = max(0, min(min(pos + 1, rec.there) - key0, kTile));
+          const int lo = static_cast<int>(max(0ll, min(static_cast<long long>(pos) - p.window + 1 - key0, static_cast<long long>(kTile))));
+          const int near = static_cast<int>(min(max(0ll, static_cast<long long>(p.sinks) - key0), static_cast<long long>(hi)));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) seen[c] = bits_of(lo - 32 * c, hi - 32 * c) | bits_of(0, near - 32 * c);
+        }
+#pragma unroll
+        for (int i = 0; i < 128; ++i) v[i] = (seen[i >> 5] >> (i & 31)) & 1u ? v[i] : 0xff800000u;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
+      float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+      // The point that a row's exponentials refer to moves when its maximum has grown past it by more than kSlack: weights stay
+      // below 2^kSlack, and O is rarely rescaled. S of this tile is there, so P V of the stream's tile before it is, too.
+      if (!begun) {
+        m = mx;
+      } else {
+        if (!(mx > m + kSlack)) mx = m;
+        if (__any_sync(0xffffffffu, mx > m && row_ok)) {
+          const float alpha = mx > m ? exp2_approx(m - mx) : 1.f;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(tmem_o + wg * 128 + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            store_tmem_32(tmem_o + wg * 128 + c, o);
+          }
+          l *= alpha;
+          m = mx;
+        }
+      }
+      begun = true;
+      const float shift = m == -INFINITY ? 0.f : -m;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 128; i += 2) {
+        const float a = exp2_approx(fmaf(__uint_as_float(v[i]), scale, shift)), b = exp2_approx(fmaf(__uint_as_float(v[i + 1]), scale, shift));
+        sum[0] += a;
+        sum[1] += b;
+        v[i / 2] = Half2<E>::pack(a, b);
+      }
+      l += sum[0] + sum[1];
+      store_tmem_32(tmem_s, &v[0]);
+      store_tmem_32(tmem_s + 32, &v[32]);
+      store_tmem_wait();
+      tc_fence_before_sync();
+      mbar_arrive(&sh.p_full[wg]);
+    }
+    if (n > 0) {
+      if (!mbar_wait_warp(&sh.o_full[wg], o_count & 1, &sh.abort_flag, kWaitNs)) return;
+      ++o_count;
+      tc_fence_after_sync();
+    }
+    // Rows of the item: of a pair both streams have their own; else the streams' results are joined, each group storing half of
+    // the columns.
+    E* const out = static_cast<E*>(p.out) + row * p.out_row + head * p.out_head;
+    const size_t ws_row = rec.slot < 0 ? 0 : static_cast<size_t>(rec.slot) * kSlotRows + (rec.pair ? wg * kTile : 0) + r;
+    float wa = 1.f, wb = 0.f, total = l, ref = m;
+    int c0 = 0, c1 = D, other = 0;
+    if (!rec.pair) {
+      sh.ml[wg][r] = make_float2(m, l);
+      mbar_arrive(&sh.x_full);
+      if (!mbar_wait_warp(&sh.x_full, x_count & 1, &sh.abort_flag, kWaitNs)) return;
+      const float2 a = sh.ml[0][r], b = sh.ml[1][r];
+      ref = fmaxf(a.x, b.x);
+      const float at = ref == -INFINITY ? 0.f : ref;
+      wa = exp2_approx(a.x - at);
+      wb = exp2_approx(b.x - at);
+      total = a.y * wa + b.y * wb;
+      c0 = wg * (D / 2);
+      c1 = c0 + D / 2;
+      other = 128;
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const uint32_t from = tmem_o + (rec.pair ? wg * 128 : 0);
+    if (works) {
+#pragma unroll 1
+      for (int c = c0; c < c1; c += 32) {
+        uint32_t a[32], b[32];
+        float f[32];
+        if (n > 0) {
+          tmem_ld_32x32(from + c, a);
+          if (other && n > 1) tmem_ld_32x32(from + other + c, b);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          f[i] = n > 0 ? __uint_as_float(a[i]) * wa : 0.f;
+          if (other && n > 1) f[i] += __uint_as_float(b[i]) * wb;
+        }
+        if (row_ok) {
+          if (rec.slot >= 0) {
+            float4* const to = reinterpret_cast<float4*>(p.ws_o + ws_row * D + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+          } else {
+            uint4* const to = reinterpret_cast<uint4*>(out + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              to[i] = make_uint4(Half2<E>::pack(f[8 * i] * inv, f[8 * i + 1] * inv), Half2<E>::pack(f[8 * i + 2] * inv, f[8 * i + 3] * inv),
+                                 Half2<E>::pack(f[8 * i + 4] * inv, f[8 * i + 5] * inv), Half2<E>::pack(f[8 * i + 6] * inv, f[8 * i + 7] * inv));
+          }
+        }
+        __syncwarp();
+      }
+      if (rec.slot >= 0 && row_ok && c0 == 0) p.ws_ml[ws_row] = make_float2(ref, total);
+    }
+    tc_fence_before_sync();
+    if (!rec.pair) {   // the accumulators and the exchange are free once both groups have read them
+      mbar_arrive(&sh.x_done);
+      if (!mbar_wait_warp(&sh.x_done, x_count & 1, &sh.abort_flag, kWaitNs)) return;
+      ++x_count;
+    }
+  }
+}
+
+template <class E, int D>
+__global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __grid_constant__ Params p) {
+  using L = Layout<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(16) Shared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  chain_release();
+  if (tid == 0) {
+    sh.abort_flag = 0;
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&sh.kv_full[i], 1);
+      mbar_init(&sh.kv_empty[i], 1);
+    }
+    for (int i = 0; i < kRecords; ++i) {
+      mbar_init(&sh.rec_full[i], 1);
+      mbar_init(&sh.rec_empty[i], 11);   // loads, products, queries and eight warps of softmax
+    }
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.o_full[i], 1);
+    }
+    mbar_init(&sh.x_full, 256);
+    mbar_init(&sh.x_done, 256);
+    mbar_init(&sh.drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem_base, 512);
+    tmem_relinquish();
+  }
+  chain_wait();
+  // The shares: each CTA adds up what all requests cost and finds where its part begins and ends.
+  long long* const prefix = reinterpret_cast<long long*>(smem);
+  int lanes = 32;
+  while (lanes > 1 && p.requests * lanes > kThreads) lanes /= 2;
+  for (int r0 = 0; r0 < p.requests; r0 += kThreads / lanes) {
+    const int r = r0 + tid / lanes;
+    Request q{0, 0, 0};
+    if (r < p.requests) q = request_of(p, r);
+    const long long cost = request_cost(p, q, tid % lanes, lanes);
+    if (r < p.requests && tid % lanes == 0) prefix[r] = cost;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    long long before = 0;
+    for (int r0 = 0; r0 < p.requests; r0 += 32) {
+      long long sum = r0 + lane < p.requests ? prefix[r0 + lane] : 0;
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += up;
+      }
+      sum += before;
+      if (r0 + lane < p.requests) prefix[r0 + lane] = sum;
+      before = __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  __syncthreads();
+  const long long total = prefix[p.requests - 1];
+  const int shares = static_cast<int>(max(min(static_cast<long long>(gridDim.x), total / kMinCost), total > 0 ? 1ll : 0ll));
+  const bool mine = static_cast<int>(blockIdx.x) < shares;
+  if (warp < 2 && mine) {
+    const Place at = place_of(p, prefix, total, shares, blockIdx.x + warp);
+    if (lane == 0) sh.place[warp] = at;
+  }
+  fence_proxy_async_smem();   // the loads write where the sums were
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (tid == 0) {   // for the kernel that joins the parts
+    int4 a = make_int4(0, 0, 0, 0), b = a;
+    if (mine && sh.place[0].t > 0) {
+      const Place at = sh.place[0];
+      const Request q = request_of(p, at.r);
+      a = make_int4(1, at.r, at.b, at.h);
+      b = make_int4(q.row0 + at.b * 2 * p.per_stream, min(2 * p.per_stream, q.rows - at.b * 2 * p.per_stream), 0, 0);
+    }
+    p.ws_meta[2 * blockIdx.x] = a;
+    p.ws_meta[2 * blockIdx.x + 1] = b;
+  }
+  uint8_t* const ring_mem = smem + 2 * L::kTileBytes;
+  // 384 threads of 168 registers: the first four warps give 96 each to the other eight (128 x 72 + 256 x 216 = 384 x 168)
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (mine) {
+      if (warp == 0) produce<D>(p, sh, ring_mem);
+      else if (warp == 1) multiply<E, D>(p, sh, smem, ring_mem);
+      else if (warp == 2) schedule(p, sh);
+      else load_queries<D>(p, sh, smem);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (mine) softmax<E, D>(p, sh, (warp - 4) >> 2);
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (tid == 0 && sh.abort_flag) atomicOr(p.status ? p.status : &g_masked_attention_status, kErrWaitTimeout);
+  if (warp == 1) tmem_dealloc(sh.tmem_base, 512);
+}
+
+// Joins the parts of the items that lie in several CTAs' shares, in order. Block (k, rows): of the item inside which CTA k's share
+// begins, if it is the first to begin there.
+template <class E, int D>
+__global__ void __launch_bounds__(256) masked_join_kernel(const __grid_constant__ Params p, int ctas) {
+  chain_release();
+  chain_wait();
+  const int k = blockIdx.x + 1, lane = threadIdx.x & 31;
+  const int4 item = p.ws_meta[2 * k], rows = p.ws_meta[2 * k + 1];
+  if (!item.x) return;
+  auto same = [&](int i) {
+    const int4 a = p.ws_meta[2 * i];
+    return a.x && a.y == item.y && a.z == item.z && a.w == item.w;
+  };
+  if (same(k - 1)) return;
+  int last = k;
+  while (last + 1 < ctas && same(last + 1)) ++last;
+  const int parts = last - k + 2;   // the tail of CTA k - 1, then the heads of k ... last
+  const int n = rows.y * p.group;
+  const bool pair = rows.y > p.per_stream;
+  for (int i = blockIdx.y * 8 + threadIdx.x / 32; i < n; i += gridDim.y * 8) {
+    const int token = i / p.group, head = i - token * p.group;
+    const int stream = pair && token >= p.per_stream;
+    const int at = stream ? kTile + (token - p.per_stream) * p.group + head : i;
+    auto slot = [&](int q) { return static_cast<size_t>(q == 0 ? 2 * (k - 1) + 1 : 2 * (k + q - 1)) * kSlotRows + at; };
+    float top = -INFINITY;
+    for (int q = lane; q < parts; q += 32) top = fmaxf(top, p.ws_ml[slot(q)].x);
+    for (int bit = 16; bit; bit >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, bit));
+    if (top == -INFINITY) top = 0.f;
+    float sum = 0.f, o[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) o[d] = 0.f;
+#pragma unroll 4
+    for (int q = 0; q < parts; ++q) {
+      const float2 ml = p.ws_ml[slot(q)];
+      const float w = exp2_approx(ml.x - top);
+      const float* const from = p.ws_o + slot(q) * D + lane * (D / 32);
+      sum += ml.y * w;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) o[d] += from[d] * w;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    E* const out = static_cast<E*>(p.out) + (rows.x + token) * p.out_row + (item.w * p.group + head) * p.out_head + lane * (D / 32);
+#pragma unroll
+    for (int d = 0; d < D / 32; d += 2) *reinterpret_cast<uint32_t*>(out + d) = Half2<E>::pack(o[d] * inv, o[d + 1] * inv);
+  }
+}
+
+struct Grid {
+  int ctas;
+  size_t o_bytes, ml_bytes, meta_bytes;
+};
+// One CTA per SM, or per tile of the largest call that the sizes allow.
+Grid grid_of(int head_dim, int sms) {
+  Grid g;
+  g.ctas = sms;
+  g.o_bytes = static_cast<size_t>(2 * g.ctas) * kSlotRows * head_dim * sizeof(float);
+  g.ml_bytes = static_cast<size_t>(2 * g.ctas) * kSlotRows * sizeof(float2);
+  g.meta_bytes = static_cast<size_t>(g.ctas) * 2 * sizeof(int4);
+  return g;
+}
+
+template <class E, int D>
+cudaError_t launch(const Params& p, const Grid& g, cudaStream_t stream) {
+  static PerDeviceOnce once;
+  cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(masked_attention_kernel<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kSmem);
+  });
+  if (e == cudaSuccess) e = launch_chained(masked_attention_kernel<E, D>, dim3(g.ctas), dim3(kThreads), Layout<D>::kSmem, stream, p);
+  if (e == cudaSuccess && g.ctas > 1) e = launch_chained(masked_join_kernel<E, D>, dim3(g.ctas - 1, 4), dim3(256), 0, stream, p, g.ctas);
+  return e;
+}
+
+int sm_count(int* sms) {
+  int device = 0;
+  MF_CUDA(cudaGetDevice(&device));
+  MF_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+  return MONOFAB_OK;
+}
+
+}  // namespace
 
 }  // namespace mf
 
 using namespace mf;
 
-extern "C" size_t monofab_masked_attention_ws_bytes(int tokens, int hq, int hkv, int head_dim) {
-  (void)tokens, (void)hq, (void)hkv, (void)head_dim;
-  return 16;
+extern "C" int64_t monofab_masked_attention_ws_bytes(int head_dim) {
+  int sms = 0;
+  if (int r = sm_count(&sms)) return r;
+  const Grid g = grid_of(head_dim, sms);
+  return static_cast<int64_t>(g.o_bytes + g.ml_bytes + g.meta_bytes);
 }
 
 extern "C" int monofab_masked_attention(const monofab_masked_attention_args* a, void* stream) {
   if (!a) return fail(MONOFAB_EINVAL, "masked_attention: NULL argument");
   if (a->tokens < 0 || a->requests < 0 || a->n_pages < 1 || a->bt_stride < 1)
     return fail(MONOFAB_EINVAL, "masked_attention: tokens=%d, requests=%d, n_pages=%d, bt_stride=%d", a->tokens, a->requests, a->n_pages, a->bt_stride);
+  if (a->requests > kMaxRequests) return fail(MONOFAB_EINVAL, "masked_attention: %d requests, at most %d a call", a->requests, kMaxRequests);
   if (a->hkv < 1 || a->hq < a->hkv || a->hq % a->hkv) return fail(MONOFAB_EINVAL, "masked_attention: hq=%d must be a multiple of hkv=%d", a->hq, a->hkv);
-  if (a->hq / a->hkv > 128) return fail(MONOFAB_EINVAL, "masked_attention: %d query heads for a KV head, at most 128", a->hq / a->hkv);
-  if (a->head_dim != 64 && a->head_dim != 128) return fail(MONOFAB_EINVAL, "masked_attention: head_dim=%d must be 64 or 128", a->head_dim);
+  const int group = a->hq / a->hkv, D = a->head_dim;
+  if (group > 128) return fail(MONOFAB_EINVAL, "masked_attention: %d query heads for a KV head, at most 128", group);
+  if (D != 64 && D != 128) return fail(MONOFAB_EINVAL, "masked_attention: head_dim=%d must be 64 or 128", D);
   if (a->page_size < 8 || a->page_size > 128 || 128 % a->page_size)
     return fail(MONOFAB_EINVAL, "masked_attention: page_size=%d must be 8, 16, 32, 64 or 128", a->page_size);
   if (static_cast<int64_t>(a->bt_stride) * a->page_size > (1ll << 30))
@@ -106,11 +964,56 @@ extern "C" int monofab_masked_attention(const monofab_masked_attention_args* a, 
     return fail(MONOFAB_EINVAL, "masked_attention: NULL argument");
   const uintptr_t at16 = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache) |
                          reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->ws);
-  if ((at16 & 15) || ((a->q_row | a->q_head | a->out_row | a->out_head) & 7) || a->q_row < 0 || a->q_head < 0)
+  if ((at16 & 15) || ((a->q_row | a->q_head | a->out_row | a->out_head) & 7) || a->q_row < 8 || a->q_head < 8)
     return fail(MONOFAB_EINVAL, "masked_attention: rows and heads of q and out, the caches and the workspace must start at multiples of 16 bytes");
-  if (a->ws_bytes < static_cast<int64_t>(monofab_masked_attention_ws_bytes(a->tokens, a->hq, a->hkv, a->head_dim)))
+  if (a->ws_bytes < 1) return fail(MONOFAB_EINVAL, "masked_attention: an empty workspace");
+  int sms = 0;
+  if (int r = sm_count(&sms)) return r;
+  const Grid g = grid_of(D, sms);
+  if (a->ws_bytes < static_cast<int64_t>(g.o_bytes + g.ml_bytes + g.meta_bytes))
     return fail(MONOFAB_EINVAL, "masked_attention: a workspace of %lld bytes is smaller than monofab_masked_attention_ws_bytes says", static_cast<long long>(a->ws_bytes));
-  MF_CUDA(launch_masked_attention(*a, static_cast<cudaStream_t>(stream)));
+  Params p{};
+  p.per_stream = kTile / group;
+  {
+    const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a->hq), static_cast<uint64_t>(a->tokens)};
+    const uint64_t strides[2] = {2 * static_cast<uint64_t>(a->q_head), 2 * static_cast<uint64_t>(a->q_row)};
+    uint32_t box[3] = {64, static_cast<uint32_t>(group), static_cast<uint32_t>(p.per_stream)};
+    if (int r = encode_map(&p.q_map, 0, a->q, 3, dims, strides, box, 128)) return r;
+    box[2] = 1;
+    if (int r = encode_map(&p.q_one_map, 0, a->q, 3, dims, strides, box, 128)) return r;
+  }
+  for (int i = 0; i < 2; ++i) {   // a page's keys of one head, both halves of the head dimension, in groups of eight keys
+    const uint64_t halves = D / 64, row = static_cast<uint64_t>(a->hkv) * D * 2;
+    const uint64_t dims[5] = {64, 8, halves * a->hkv, static_cast<uint64_t>(a->page_size / 8), static_cast<uint64_t>(a->n_pages)};
+    const uint64_t strides[4] = {row, 128, 8 * row, static_cast<uint64_t>(a->page_size) * row};
+    const uint32_t box[5] = {64, 8, static_cast<uint32_t>(halves), static_cast<uint32_t>(a->page_size / 8), 1};
+    if (int r = encode_map(i ? &p.v_map : &p.k_map, 0, i ? a->v_cache : a->k_cache, 5, dims, strides, box, 128)) return r;
+  }
+  p.block_table = a->block_table;
+  p.q_start = a->q_start;
+  p.kv_len = a->kv_len;
+  p.tree = a->tree;
+  p.out = a->out;
+  p.status = a->status;
+  p.ws_o = static_cast<float*>(a->ws);
+  p.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(a->ws) + g.o_bytes);
+  p.ws_meta = reinterpret_cast<int4*>(static_cast<char*>(a->ws) + g.o_bytes + g.ml_bytes);
+  p.out_row = a->out_row;
+  p.out_head = a->out_head;
+  p.tokens = a->tokens;
+  p.requests = a->requests;
+  p.hkv = a->hkv;
+  p.group = group;
+  p.page = a->page_size;
+  p.n_pages = a->n_pages;
+  p.bt_stride = a->bt_stride;
+  p.words = a->words;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  p.scale_log2 = a->scale * 1.44269504088896340736f;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->fp16) MF_CUDA((D == 64 ? launch<__half, 64>(p, g, st) : launch<__half, 128>(p, g, st)));
+  else MF_CUDA((D == 64 ? launch<__nv_bfloat16, 64>(p, g, st) : launch<__nv_bfloat16, 128>(p, g, st)));
   return MONOFAB_OK;
 }
 

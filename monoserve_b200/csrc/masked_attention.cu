@@ -167,6 +167,14 @@ __device__ __forceinline__ void store_tmem_32(uint32_t taddr, const uint32_t* r)
         "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void store_tmem_16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void store_tmem_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -203,6 +211,13 @@ __device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
   lo = max(lo, 0), hi = min(hi, 32);
   if (lo >= hi) return 0u;
   return (0xffffffffu >> (32 - (hi - lo))) << lo;
+}
+
+// Scores whose bit is not set are as low as can be.
+template <int N>
+__device__ __forceinline__ void hide(uint32_t* v, uint32_t seen) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = seen >> i & 1u ? v[i] : 0xff800000u;
 }
 
 // ---------------------------------------------------------------------------------------------------- the shares
@@ -606,18 +621,14 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
         continue;
       }
       const int key0 = rec.tile_key(rec.t0 + j);
-      uint32_t v[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32(tmem_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
-      tmem_ld_wait();
       bool full;
+      uint32_t seen[4];
       if (p.tree) full = key0 + kTile <= min(rec.past, rec.there);
       else
         full = key0 + kTile - 1 <= pos_first && key0 + kTile <= rec.there &&
                (static_cast<long long>(key0) > static_cast<long long>(pos_last) - p.window || key0 + kTile <= p.sinks);
       if (!full) {
-        // what the row sees of the tile, as 128 bits
-        uint32_t seen[4];
+        // what the row sees of the tile
         if (p.tree) {
           const int32_t* const words = p.tree + static_cast<size_t>(row_ok ? row : rec.row0) * p.words;
 #pragma unroll
@@ -634,13 +645,24 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) seen[c] = bits_of(lo - 32 * c, hi - 32 * c) | bits_of(0, near - 32 * c);
         }
-#pragma unroll
-        for (int i = 0; i < 128; ++i) v[i] = (seen[i >> 5] >> (i & 31)) & 1u ? v[i] : 0xff800000u;
       }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 64) {
+        uint32_t v[64];
+        tmem_ld_32x32(tmem_s + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        tmem_ld_32x32(tmem_s + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        tmem_ld_wait();
+        if (!full) {
+          hide<32>(&v[0], c ? seen[2] : seen[0]);
+          hide<32>(&v[32], c ? seen[3] : seen[1]);
+        }
+        float top[4] = {mx, mx, mx, mx};
 #pragma unroll
-      for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
-      float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+        for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
+        mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      }
+      mx *= scale;
       // The point that a row's exponentials refer to moves when its maximum has grown past it by more than kSlack: weights stay
       // below 2^kSlack, and O is rarely rescaled. S of this tile is there, so P V of the stream's tile before it is, too.
       if (!begun) {
@@ -665,16 +687,22 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
       begun = true;
       const float shift = m == -INFINITY ? 0.f : -m;
       float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32(tmem_s + c, v);
+        tmem_ld_wait();
+        if (!full) hide<32>(v, c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3]));
 #pragma unroll
-      for (int i = 0; i < 128; i += 2) {
-        const float a = exp2_approx(fmaf(__uint_as_float(v[i]), scale, shift)), b = exp2_approx(fmaf(__uint_as_float(v[i + 1]), scale, shift));
-        sum[0] += a;
-        sum[1] += b;
-        v[i / 2] = Half2<E>::pack(a, b);
+        for (int i = 0; i < 32; i += 2) {
+          const float a = exp2_approx(fmaf(__uint_as_float(v[i]), scale, shift)), b = exp2_approx(fmaf(__uint_as_float(v[i + 1]), scale, shift));
+          sum[0] += a;
+          sum[1] += b;
+          v[i / 2] = Half2<E>::pack(a, b);
+        }
+        store_tmem_16(tmem_s + c / 2, v);
       }
       l += sum[0] + sum[1];
-      store_tmem_32(tmem_s, &v[0]);
-      store_tmem_32(tmem_s + 32, &v[32]);
       store_tmem_wait();
       tc_fence_before_sync();
       mbar_arrive(&sh.p_full[wg]);
@@ -830,9 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     p.ws_meta[2 * blockIdx.x + 1] = b;
   }
   uint8_t* const ring_mem = smem + 2 * L::kTileBytes;
-  // 384 threads of 168 registers: the first four warps give 96 each to the other eight (128 x 72 + 256 x 216 = 384 x 168)
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (mine) {
       if (warp == 0) produce<D>(p, sh, ring_mem);
       else if (warp == 1) multiply<E, D>(p, sh, smem, ring_mem);
@@ -840,7 +866,6 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
       else load_queries<D>(p, sh, smem);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     if (mine) softmax<E, D>(p, sh, (warp - 4) >> 2);
   }
   __syncwarp();

@@ -50,6 +50,15 @@ struct Params {
   float scale_log2;
 };
 
+// A bounded wait by the whole warp, which goes on or gives up as one (ptx.cuh); what happens when the phase is not there yet is kept out of
+// the callers' code.
+__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, int* abort_flag) {
+  return mbar_wait_warp(bar, parity, abort_flag, kWaitNs);
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_longer(bar, parity, abort_flag);
+}
+
 // A request as the device sees it.
 struct Request {
   int row0, rows, kv_len;
@@ -116,7 +125,7 @@ struct Layout {
 
 struct Shared {
   uint64_t kv_full[10], kv_empty[10], rec_full[kRecords], rec_empty[kRecords];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], x_full, x_done, drain;
+  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], x_full, x_done, drain[2];
   uint32_t tmem_base;
   int abort_flag;
   Place place[2];
@@ -126,9 +135,8 @@ struct Shared {
 
 // Descriptors: Q rows of 128 bytes a half, halves 16 KB apart; K and V tiles in groups of eight keys, the halves of a group
 // 1 KB apart (one TMA box of a page delivers both).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 | static_cast<uint64_t>(stride >> 4) << 32 |
-         static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+__device__ __forceinline__ uint64_t smem_desc(uint32_t low, uint32_t stride) {   // low: address / 16 | leading offset / 16 << 16
+  return static_cast<uint64_t>((stride >> 4) | 1u << 14 | 2u << 29) << 32 | low;
 }
 
 // D[tmem] (+)= A[tmem] * B[smem]; issued by one thread.
@@ -285,9 +293,12 @@ __device__ Place place_of(const Params& p, const long long* prefix, long long to
   return at;
 }
 
-// Writes the records of the items from place[0] to place[1].
-__device__ void schedule(const Params& p, Shared& sh) {
+// Writes the records of the items from place[0] to place[1], and loads each one's queries once the scores of the one before have read theirs.
+template <int D>
+__device__ void schedule(const Params& p, Shared& sh, uint8_t* q_mem) {
+  using L = Layout<D>;
   const int lane = threadIdx.x & 31;
+  uint32_t q_uses = 0;
   Place at = sh.place[0];
   const Place end = sh.place[1];
   int seen_from = -1;
@@ -339,14 +350,29 @@ __device__ void schedule(const Params& p, Shared& sh) {
       }
     }
     const int slot = n % kRecords;
-    if (n >= kRecords && !mbar_wait_warp(&sh.rec_empty[slot], (n / kRecords - 1) & 1, &sh.abort_flag, kWaitNs)) return;
+    if (n >= kRecords && !wait_for(&sh.rec_empty[slot], (n / kRecords - 1) & 1, &sh.abort_flag)) break;
     if (lane == 0) {
       sh.rec[slot] = rec;
       mbar_arrive(&sh.rec_full[slot]);
     }
     __syncwarp();
-    if (rec.pair < 0) return;
+    if (rec.pair < 0) break;
+    if (rec.t0 == rec.t1) continue;
+    if (q_uses > 0 && !wait_for(&sh.q_empty, (q_uses - 1) & 1, &sh.abort_flag)) break;
+    ++q_uses;
+    if (lane == 0) {
+      const bool one = rec.tokens == 1;
+      const CUtensorMap* const map = one ? &p.q_one_map : &p.q_map;
+      mbar_arrive_expect_tx(&sh.q_full, (1 + rec.pair) * L::kHalves * p.group * (one ? 1 : p.per_stream) * 128);
+      for (int s = 0; s <= rec.pair; ++s)
+        for (int h = 0; h < L::kHalves; ++h)
+          load_box_3d(q_mem + s * L::kTileBytes + h * (kTile * 128), map, &sh.q_full, 64 * h, rec.head * p.group, rec.row0 + s * p.per_stream);
+    }
+    __syncwarp();
   }
+  // however it ended, the last queries have landed before the CTA's memory is given up
+  int ignored = 0;
+  if (q_uses > 0) wait_for(&sh.q_full, (q_uses - 1) & 1, &ignored);
 }
 
 // The next record, by every warp of a role alike. False: no more.
@@ -354,7 +380,7 @@ struct Records {
   int n = 0;
   __device__ __forceinline__ bool next(Shared& sh, Record& rec) {
     const int slot = n % kRecords;
-    if (!mbar_wait_warp(&sh.rec_full[slot], (n / kRecords) & 1, &sh.abort_flag, kWaitNs)) return false;
+    if (!wait_for(&sh.rec_full[slot], (n / kRecords) & 1, &sh.abort_flag)) return false;
     rec = sh.rec[slot];
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.rec_empty[slot]);
@@ -404,7 +430,7 @@ __device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
     int last_page = 0;
     bool last_there = false;
     auto load = [&](const CUtensorMap* map, int page, bool wanted) {
-      if (!mbar_wait_warp(&sh.kv_empty[ring.stage], ring.phase ^ 1, &sh.abort_flag, kWaitNs)) return false;
+      if (!wait_for(&sh.kv_empty[ring.stage], ring.phase ^ 1, &sh.abort_flag)) return false;
       const uint32_t which = __ballot_sync(0xffffffffu, wanted);
       if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[ring.stage], __popc(which) * page_bytes);
       __syncwarp();
@@ -432,162 +458,109 @@ __device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
   // however it ended, the last loads have landed before the CTA's memory is given up
   for (uint32_t i = loads > L::kStages ? loads - L::kStages : 0; i < loads; ++i) {
     int ignored = 0;
-    mbar_wait_warp(&sh.kv_full[i % L::kStages], (i / L::kStages) & 1, &ignored, kWaitNs);
+    wait_for(&sh.kv_full[i % L::kStages], (i / L::kStages) & 1, &ignored);
   }
 }
 
-template <int D>
-__device__ void load_queries(const Params& p, Shared& sh, uint8_t* q_mem) {
-  using L = Layout<D>;
-  const int lane = threadIdx.x & 31;
-  Records records;
-  Record rec;
-  int uses = 0;
-  while (records.next(sh, rec)) {
-    if (rec.t0 == rec.t1) continue;
-    if (uses > 0 && !mbar_wait_warp(&sh.q_empty, (uses - 1) & 1, &sh.abort_flag, kWaitNs)) break;
-    ++uses;
-    if (lane == 0) {
-      const bool one = rec.tokens == 1;
-      const CUtensorMap* const map = one ? &p.q_one_map : &p.q_map;
-      const int rows = p.group * (one ? 1 : p.per_stream);
-      mbar_arrive_expect_tx(&sh.q_full, (1 + rec.pair) * L::kHalves * rows * 128);
-      for (int s = 0; s <= rec.pair; ++s)
-        for (int h = 0; h < L::kHalves; ++h)
-          load_box_3d(q_mem + s * L::kTileBytes + h * (kTile * 128), map, &sh.q_full, 64 * h, rec.head * p.group, rec.row0 + s * p.per_stream);
-    }
-    __syncwarp();
-  }
-  int ignored = 0;
-  if (uses > 0) mbar_wait_warp(&sh.q_full, (uses - 1) & 1, &ignored, kWaitNs);
-}
-
+// The products of stream x, by a warp of its own: each stream's chain of scores, weights and values has nothing to wait for in the
+// other's. In a pair both read every stage; else a warp only says of the other stream's stages that it does not need them.
 template <class E, int D>
-__device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* ring_mem) {
+__device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* ring_mem, int x) {
   using L = Layout<D>;
   const int lane = threadIdx.x & 31;
   const bool leader = elect_one();
-  const uint32_t tmem = sh.tmem_base;
+  const uint32_t tmem_s = __shfl_sync(0xffffffffu, sh.tmem_base, 0) + x * 128, tmem_o = tmem_s + 256;
   constexpr uint32_t idesc_s = idesc_of<E>(kTile), idesc_o = idesc_of<E>(D) | (1u << 16);   // V is MN-major
   Ring<L::kStages> ring;
   Records records;
   Record rec{};
-  int q_uses = 0;
-  uint32_t p_count[2] = {0, 0};
-  auto wait_stage = [&] { return mbar_wait_warp(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag, kWaitNs); };
-  auto scores = [&](int x, int q_tile, int stage) {   // S[x] = Q K^T
-    if (!leader) return;
-    const uint32_t q = smem_u32(q_mem) + q_tile * L::kTileBytes, k = smem_u32(ring_mem) + stage * L::kTileBytes;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-      umma_bf16(tmem + x * 128, smem_desc(q + (i >> 2) * (kTile * 128) + (i & 3) * 32, 0, 1024),
-                smem_desc(k + (i >> 2) * 1024 + (i & 3) * 32, 0, L::kGroupBytes), idesc_s, i != 0);
-    umma_commit(&sh.s_full[x]);
-  };
-  auto values = [&](int x, int stage, bool accumulate) {   // O[x] (+)= P[x] V
-    if (!leader) return;
-    const uint32_t v = smem_u32(ring_mem) + stage * L::kTileBytes;
-#pragma unroll
-    for (int i = 0; i < kTile / 16; ++i)
-      umma_tmem_a(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, smem_desc(v + i * 2 * L::kGroupBytes, 1024, L::kGroupBytes), idesc_o,
-                  accumulate || i != 0);
-  };
-  auto wait_weights = [&](int x) {
-    const bool ok = mbar_wait_warp(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag, kWaitNs);
-    ++p_count[x];
+  uint32_t q_count = 0, p_count = 0;
+  // S = Q K^T of the ring's next stage; `last`: of the item
+  auto scores = [&](int q_tile, bool last) {
+    if (!wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag)) return false;
     tc_fence_after_sync();
-    return ok;
-  };
-  // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none.
-  auto clean = [&](int stage, int key0) {
-    if (key0 + kTile <= rec.hi && (key0 >= rec.lo || key0 + kTile <= rec.near)) return;
-    uint8_t* const v = ring_mem + stage * L::kTileBytes;
-    for (int i = lane / 8; i < kTile * L::kHalves; i += 4) {
-      const int k = i / L::kHalves;
-      if (!some_row_sees(rec, key0 + k))
-        *reinterpret_cast<uint4*>(v + (k >> 3) * L::kGroupBytes + (i % L::kHalves) * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    const uint32_t q = (smem_u32(q_mem) + q_tile * L::kTileBytes) >> 4, k = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4;
+    if (leader) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        umma_bf16(tmem_s, smem_desc(q + (i >> 2) * (kTile * 8) + (i & 3) * 2, 1024), smem_desc(k + (i >> 2) * 64 + (i & 3) * 2, L::kGroupBytes), idesc_s,
+                  i != 0);
+      umma_commit(&sh.s_full[x]);
+      umma_commit(&sh.kv_empty[ring.stage]);
+      if (last) umma_commit(&sh.q_empty);
     }
-    fence_proxy_async_smem();
-    __syncwarp();
+    ring.advance();
+    return true;
+  };
+  // O (+)= P V of the ring's next stage
+  auto values = [&](int t, bool accumulate) {
+    if (!wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag)) return false;
+    // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none. (In a pair both warps write
+    // the same zeros.)
+    const int key0 = rec.tile_key(t);
+    if (!(key0 + kTile <= rec.hi && (key0 >= rec.lo || key0 + kTile <= rec.near))) {
+      uint8_t* const v = ring_mem + ring.stage * L::kTileBytes;
+      for (int i = lane / 8; i < kTile * L::kHalves; i += 4) {
+        const int k = i / L::kHalves;
+        if (!some_row_sees(rec, key0 + k))
+          *reinterpret_cast<uint4*>(v + (k >> 3) * L::kGroupBytes + (i % L::kHalves) * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    if (!wait_for(&sh.p_full[x], p_count & 1, &sh.abort_flag)) return false;
+    ++p_count;
+    tc_fence_after_sync();
+    const uint32_t v = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4 | 64u << 16;
+    if (leader) {
+#pragma unroll
+      for (int i = 0; i < kTile / 16; ++i)
+        umma_tmem_a(tmem_o, tmem_s + 8 * i, smem_desc(v + i * (L::kGroupBytes / 8), L::kGroupBytes), idesc_o, accumulate || i != 0);
+      umma_commit(&sh.kv_empty[ring.stage]);
+    }
+    ring.advance();
+    return true;
+  };
+  auto pass = [&] {   // the other stream's stage
+    if (!wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag)) return false;
+    if (lane == 0) mbar_arrive(&sh.kv_empty[ring.stage]);
+    ring.advance();
+    return true;
   };
   auto run = [&] {
     while (records.next(sh, rec)) {
       const int n = rec.t1 - rec.t0;
       if (n == 0) continue;
-      if (!mbar_wait_warp(&sh.q_full, q_uses & 1, &sh.abort_flag, kWaitNs)) return;
-      ++q_uses;
-      if (!wait_stage()) return;
-      tc_fence_after_sync();
-      scores(0, 0, ring.stage);
+      if (!wait_for(&sh.q_full, q_count & 1, &sh.abort_flag)) return;
+      ++q_count;
       if (rec.pair) {
-        scores(1, 1, ring.stage);
-        if (leader) umma_commit(&sh.kv_empty[ring.stage]);
-        if (leader && n == 1) umma_commit(&sh.q_empty);
-        ring.advance();
+        if (!scores(x, n == 1)) return;
         for (int j = 0; j < n; ++j) {
-          if (!wait_stage()) return;
-          const int v_stage = ring.stage;
-          clean(v_stage, rec.tile_key(rec.t0 + j));
-          ring.advance();
-          if (!wait_weights(0)) return;
-          values(0, v_stage, j > 0);
-          if (j + 1 < n) {
-            if (!wait_stage()) return;
-            tc_fence_after_sync();
-            scores(0, 0, ring.stage);
-          } else if (leader) {
-            umma_commit(&sh.o_full[0]);
-          }
-          if (!wait_weights(1)) return;
-          values(1, v_stage, j > 0);
-          if (leader) umma_commit(&sh.kv_empty[v_stage]);
-          if (j + 1 < n) {
-            scores(1, 1, ring.stage);
-            if (leader) umma_commit(&sh.kv_empty[ring.stage]);
-            if (leader && j + 2 == n) umma_commit(&sh.q_empty);
-            ring.advance();
-          } else if (leader) {
-            umma_commit(&sh.o_full[1]);
-          }
+          if (!values(rec.t0 + j, j > 0)) return;
+          if (j + 1 < n && !scores(x, j + 2 == n)) return;
         }
-        continue;
-      }
-      if (leader) umma_commit(&sh.kv_empty[ring.stage]);
-      ring.advance();
-      if (n > 1) {
-        if (!wait_stage()) return;
-        tc_fence_after_sync();
-        scores(1, 0, ring.stage);
-        if (leader) umma_commit(&sh.kv_empty[ring.stage]);
-        ring.advance();
-      }
-      if (leader && n <= 2) umma_commit(&sh.q_empty);
-      for (int j = 0; j < n; ++j) {
-        const int x = j & 1;
-        if (!wait_stage()) return;
-        clean(ring.stage, rec.tile_key(rec.t0 + j));
-        if (!wait_weights(x)) return;
-        values(x, ring.stage, j > 1);
-        if (leader) umma_commit(&sh.kv_empty[ring.stage]);
-        ring.advance();
-        if (j + 2 < n) {
-          if (!wait_stage()) return;
-          tc_fence_after_sync();
-          scores(x, 0, ring.stage);
-          if (leader) umma_commit(&sh.kv_empty[ring.stage]);
-          if (leader && j + 3 == n) umma_commit(&sh.q_empty);
-          ring.advance();
+      } else {
+        // stages: K 0, K 1, V 0, K 2, V 1, ... K n - 1, V n - 2, V n - 1
+        const int mine = (n + 1 - x) / 2;   // tiles of this stream
+        if (x == 0 ? !scores(0, mine == 1) : !pass()) return;
+        if (n > 1 && (x == 1 ? !scores(0, mine == 1) : !pass())) return;
+        if (mine == 0 && leader) umma_commit(&sh.q_empty);
+        for (int j = 0; j < n; ++j) {
+          const bool own = (j & 1) == x;
+          if (own ? !values(rec.t0 + j, j > 1) : !pass()) return;
+          if (j + 2 < n && (own ? !scores(0, j + 4 >= n) : !pass())) return;
         }
       }
-      if (leader) umma_commit(&sh.o_full[0]);
-      if (leader) umma_commit(&sh.o_full[1]);
+      // Only where the stream has tiles: its softmax holds this warp back then. Without, it could complete the barrier twice before
+      // anybody looks.
+      if (leader && (rec.pair || n > x)) umma_commit(&sh.o_full[x]);
     }
   };
   run();
   // whatever ended the loop: nothing of this warp is in flight when it leaves
-  if (leader) umma_commit(&sh.drain);
+  if (leader) umma_commit(&sh.drain[x]);
   int ignored = 0;
-  mbar_wait_warp(&sh.drain, 0, &ignored, kWaitNs);
+  wait_for(&sh.drain[x], 0, &ignored);
 }
 
 template <class E, int D>
@@ -612,7 +585,7 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
     float m = -INFINITY, l = 0.f;
     bool begun = false;
     for (int j = rec.pair ? 0 : wg; j < n; j += rec.pair ? 1 : 2) {
-      if (!mbar_wait_warp(&sh.s_full[wg], s_count & 1, &sh.abort_flag, kWaitNs)) return;
+      if (!wait_for(&sh.s_full[wg], s_count & 1, &sh.abort_flag)) return;
       ++s_count;
       tc_fence_after_sync();
       if (!works) {   // no row of this warp exists
@@ -707,8 +680,8 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
       tc_fence_before_sync();
       mbar_arrive(&sh.p_full[wg]);
     }
-    if (n > 0) {
-      if (!mbar_wait_warp(&sh.o_full[wg], o_count & 1, &sh.abort_flag, kWaitNs)) return;
+    if (n > (rec.pair ? 0 : wg)) {   // the stream has tiles
+      if (!wait_for(&sh.o_full[wg], o_count & 1, &sh.abort_flag)) return;
       ++o_count;
       tc_fence_after_sync();
     }
@@ -721,7 +694,8 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
     if (!rec.pair) {
       sh.ml[wg][r] = make_float2(m, l);
       mbar_arrive(&sh.x_full);
-      if (!mbar_wait_warp(&sh.x_full, x_count & 1, &sh.abort_flag, kWaitNs)) return;
+      if (!wait_for(&sh.x_full, x_count & 1, &sh.abort_flag)) return;
+      tc_fence_after_sync();   // the other stream's products are there, too: its threads have waited for them
       const float2 a = sh.ml[0][r], b = sh.ml[1][r];
       ref = fmaxf(a.x, b.x);
       const float at = ref == -INFINITY ? 0.f : ref;
@@ -769,7 +743,7 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
     tc_fence_before_sync();
     if (!rec.pair) {   // the accumulators and the exchange are free once both groups have read them
       mbar_arrive(&sh.x_done);
-      if (!mbar_wait_warp(&sh.x_done, x_count & 1, &sh.abort_flag, kWaitNs)) return;
+      if (!wait_for(&sh.x_done, x_count & 1, &sh.abort_flag)) return;
       ++x_count;
     }
   }
@@ -786,22 +760,22 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     sh.abort_flag = 0;
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&sh.kv_full[i], 1);
-      mbar_init(&sh.kv_empty[i], 1);
+      mbar_init(&sh.kv_empty[i], 2);   // both streams' products
     }
     for (int i = 0; i < kRecords; ++i) {
       mbar_init(&sh.rec_full[i], 1);
       mbar_init(&sh.rec_empty[i], 11);   // loads, products, queries and eight warps of softmax
     }
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.q_empty, 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 128);
       mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.drain[i], 1);
     }
     mbar_init(&sh.x_full, 256);
     mbar_init(&sh.x_done, 256);
-    mbar_init(&sh.drain, 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -861,9 +835,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
   if (warp < 4) {
     if (mine) {
       if (warp == 0) produce<D>(p, sh, ring_mem);
-      else if (warp == 1) multiply<E, D>(p, sh, smem, ring_mem);
-      else if (warp == 2) schedule(p, sh);
-      else load_queries<D>(p, sh, smem);
+      else if (warp == 2) schedule<D>(p, sh, smem);
+      else multiply<E, D>(p, sh, smem, ring_mem, warp >> 1);
     }
   } else {
     if (mine) softmax<E, D>(p, sh, (warp - 4) >> 2);

@@ -29,6 +29,7 @@ constexpr int kSlotRows = 2 * kTile;
 constexpr int kMaxRequests = 16384;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr float kSlack = 8.f;
+constexpr int kByFma = 4;           // weights of 32 worked out by multiplications
 
 // Where a call that names no status word leaves its bits.
 __device__ int g_masked_attention_status;
@@ -125,7 +126,7 @@ struct Layout {
 
 struct Shared {
   uint64_t kv_full[10], kv_empty[10], rec_full[kRecords], rec_empty[kRecords];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], x_full, x_done, drain[2];
+  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], x_full, x_done, drain;
   uint32_t tmem_base;
   int abort_flag;
   Place place[2];
@@ -164,17 +165,6 @@ __device__ __forceinline__ void load_box_5d(void* smem, const void* map, uint64_
                : "r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(c2), "r"(c4)
                : "memory");
 }
-__device__ __forceinline__ void store_tmem_32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      :
-      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 __device__ __forceinline__ void store_tmem_16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -191,11 +181,51 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two 32-bit values as one operand of the packed instructions.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 parts_of(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <class E>
 struct Half2;
 template <>
 struct Half2<__nv_bfloat16> {
   static constexpr uint32_t kFormat = 1;
+  // 2^x on [-1/2, 1/2] with the least relative error of its degree, 7.5e-5: a fiftieth of the rounding to bf16 that follows
+  static __device__ __forceinline__ Pair power(Pair f) {
+    Pair y = pair_of(0.05517166852951f, 0.05517166852951f);
+    y = fma2(y, f, pair_of(0.24261112511158f, 0.24261112511158f));
+    y = fma2(y, f, pair_of(0.69326096773148f, 0.69326096773148f));
+    return fma2(y, f, pair_of(0.99992805719376f, 0.99992805719376f));
+  }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -204,6 +234,14 @@ struct Half2<__nv_bfloat16> {
 template <>
 struct Half2<__half> {
   static constexpr uint32_t kFormat = 0;
+  // one degree more, 2.6e-6, for fp16's smaller rounding
+  static __device__ __forceinline__ Pair power(Pair f) {
+    Pair y = pair_of(0.00957010220736f, 0.00957010220736f);
+    y = fma2(y, f, pair_of(0.05591785907745f, 0.05591785907745f));
+    y = fma2(y, f, pair_of(0.24024744331837f, 0.24024744331837f));
+    y = fma2(y, f, pair_of(0.69312179088593f, 0.69312179088593f));
+    return fma2(y, f, pair_of(0.99999928474426f, 0.99999928474426f));
+  }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -212,6 +250,40 @@ struct Half2<__half> {
 template <class E>
 __host__ __device__ constexpr uint32_t idesc_of(int n) {   // fp32 accumulators, M = 128
   return (1u << 4) | (Half2<E>::kFormat << 7) | (Half2<E>::kFormat << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+// 2^x of two values by multiplications: x = n + f with n whole, 2^f by a polynomial, n added to its exponent. Zero below 2^-126.
+template <class E>
+__device__ __forceinline__ float2 exp2_by_fma(Pair x) {
+  const float2 v = parts_of(x);
+  x = pair_of(max_or_nan(v.x, -126.f), max_or_nan(v.y, -126.f));
+  const float big = 12582912.f;   // 3 * 2^22: sums with it are rounded to whole numbers
+  const Pair t = add2(x, pair_of(big, big));
+  const Pair f = fma2(add2(t, pair_of(-big, -big)), pair_of(-1.f, -1.f), x);
+  const float2 y = parts_of(Half2<E>::power(f)), n = parts_of(t);
+  return make_float2(v.x < -126.f ? 0.f : __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
+                     v.y < -126.f ? 0.f : __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// The weights of 32 scores, packed, and added to `sum`. kByFma of them are worked out by multiplications: the special-function unit
+// gives 16 a cycle and SM, as long for a tile as its matrix products. (None: long trees 466 us, window prompts 169; 4: 457, 166;
+// 8: 458, 167, and decode batches 1 % longer.)
+template <class E>
+__device__ __forceinline__ void weigh(const uint32_t (&v)[32], float scale, float shift, Pair& sum, uint32_t (&out)[16]) {
+  const Pair scales = pair_of(scale, scale), shifts = pair_of(shift, shift);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const Pair x = fma2(pair_of(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scales, shifts);
+    float2 w;
+    if (i * kByFma / 32 != (i + 1) * kByFma / 32) {   // spread over them
+      w = exp2_by_fma<E>(x);
+    } else {
+      const float2 a = parts_of(x);
+      w = make_float2(exp2_approx(a.x), exp2_approx(a.y));
+    }
+    sum = add2(sum, pair_of(w.x, w.y));
+    out[i] = Half2<E>::pack(w.x, w.y);
+  }
 }
 
 // Bits of [lo, hi) in a word.
@@ -375,17 +447,18 @@ __device__ void schedule(const Params& p, Shared& sh, uint8_t* q_mem) {
   if (q_uses > 0) wait_for(&sh.q_full, (q_uses - 1) & 1, &ignored);
 }
 
-// The next record, by every warp of a role alike. False: no more.
+// The records one after the other, by every warp of a role alike. What a warp got is its own until it asks for the next one.
 struct Records {
   int n = 0;
-  __device__ __forceinline__ bool next(Shared& sh, Record& rec) {
+  __device__ __forceinline__ const Record* next(Shared& sh) {
+    if (n > 0) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.rec_empty[(n - 1) % kRecords]);
+    }
     const int slot = n % kRecords;
-    if (!wait_for(&sh.rec_full[slot], (n / kRecords) & 1, &sh.abort_flag)) return false;
-    rec = sh.rec[slot];
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.rec_empty[slot]);
+    if (!wait_for(&sh.rec_full[slot], (n / kRecords) & 1, &sh.abort_flag)) return nullptr;
     ++n;
-    return rec.pair >= 0;
+    return sh.rec[slot].pair >= 0 ? &sh.rec[slot] : nullptr;
   }
 };
 
@@ -415,9 +488,9 @@ __device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
   Ring<L::kStages> ring;
   uint32_t loads = 0;
   Records records;
-  Record rec;
   auto run = [&] {
-  while (records.next(sh, rec)) {
+  while (const Record* const got = records.next(sh)) {
+    const Record rec = *got;   // in registers: the loops below would read it again behind every barrier
     const int n = rec.t1 - rec.t0, lead = rec.pair ? 0 : 1;   // K runs one tile ahead of V where the streams take alternate tiles
     const int32_t* const table = p.block_table + static_cast<size_t>(rec.req) * p.bt_stride;
     int ahead = 0;   // this lane's page of the tile of `step`, and whether some row sees a key of it
@@ -462,105 +535,110 @@ __device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
   }
 }
 
-// The products of stream x, by a warp of its own: each stream's chain of scores, weights and values has nothing to wait for in the
-// other's. In a pair both read every stage; else a warp only says of the other stream's stages that it does not need them.
+// The products of both streams, by one warp: it keeps them a step apart, so that one stream's products run under the other's softmax.
 template <class E, int D>
-__device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* ring_mem, int x) {
+__device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* ring_mem) {
   using L = Layout<D>;
   const int lane = threadIdx.x & 31;
   const bool leader = elect_one();
-  const uint32_t tmem_s = __shfl_sync(0xffffffffu, sh.tmem_base, 0) + x * 128, tmem_o = tmem_s + 256;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem_base, 0);
   constexpr uint32_t idesc_s = idesc_of<E>(kTile), idesc_o = idesc_of<E>(D) | (1u << 16);   // V is MN-major
   Ring<L::kStages> ring;
   Records records;
-  Record rec{};
-  uint32_t q_count = 0, p_count = 0;
-  // S = Q K^T of the ring's next stage; `last`: of the item
-  auto scores = [&](int q_tile, bool last) {
-    if (!wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag)) return false;
-    tc_fence_after_sync();
-    const uint32_t q = (smem_u32(q_mem) + q_tile * L::kTileBytes) >> 4, k = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4;
-    if (leader) {
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-        umma_bf16(tmem_s, smem_desc(q + (i >> 2) * (kTile * 8) + (i & 3) * 2, 1024), smem_desc(k + (i >> 2) * 64 + (i & 3) * 2, L::kGroupBytes), idesc_s,
-                  i != 0);
-      umma_commit(&sh.s_full[x]);
-      umma_commit(&sh.kv_empty[ring.stage]);
-      if (last) umma_commit(&sh.q_empty);
-    }
-    ring.advance();
-    return true;
+  uint32_t q_count = 0, p_count[2] = {0, 0};
+  auto wait_stage = [&] { return wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag); };
+  auto release = [&](int stage) {
+    if (leader) umma_commit(&sh.kv_empty[stage]);
   };
-  // O (+)= P V of the ring's next stage
-  auto values = [&](int t, bool accumulate) {
-    if (!wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag)) return false;
-    // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none. (In a pair both warps write
-    // the same zeros.)
-    const int key0 = rec.tile_key(t);
-    if (!(key0 + kTile <= rec.hi && (key0 >= rec.lo || key0 + kTile <= rec.near))) {
-      uint8_t* const v = ring_mem + ring.stage * L::kTileBytes;
-      for (int i = lane / 8; i < kTile * L::kHalves; i += 4) {
-        const int k = i / L::kHalves;
-        if (!some_row_sees(rec, key0 + k))
-          *reinterpret_cast<uint4*>(v + (k >> 3) * L::kGroupBytes + (i % L::kHalves) * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-    }
-    if (!wait_for(&sh.p_full[x], p_count & 1, &sh.abort_flag)) return false;
-    ++p_count;
+  auto scores = [&](int x, int q_tile) {   // S[x] = Q K^T of the ring's stage
+    if (!leader) return;
+    const uint32_t q = (smem_u32(q_mem) + q_tile * L::kTileBytes) >> 4, k = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      umma_bf16(tmem + x * 128, smem_desc(q + (i >> 2) * (kTile * 8) + (i & 3) * 2, 1024), smem_desc(k + (i >> 2) * 64 + (i & 3) * 2, L::kGroupBytes), idesc_s,
+                i != 0);
+    umma_commit(&sh.s_full[x]);
+  };
+  auto values = [&](int x, int stage, bool accumulate) {   // O[x] (+)= P[x] V
+    if (!wait_for(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag)) return false;
+    ++p_count[x];
     tc_fence_after_sync();
-    const uint32_t v = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4 | 64u << 16;
+    const uint32_t v = (smem_u32(ring_mem) + stage * L::kTileBytes) >> 4 | 64u << 16;
     if (leader) {
 #pragma unroll
       for (int i = 0; i < kTile / 16; ++i)
-        umma_tmem_a(tmem_o, tmem_s + 8 * i, smem_desc(v + i * (L::kGroupBytes / 8), L::kGroupBytes), idesc_o, accumulate || i != 0);
-      umma_commit(&sh.kv_empty[ring.stage]);
+        umma_tmem_a(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, smem_desc(v + i * (L::kGroupBytes / 8), L::kGroupBytes), idesc_o, accumulate || i != 0);
     }
-    ring.advance();
     return true;
   };
-  auto pass = [&] {   // the other stream's stage
-    if (!wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag)) return false;
-    if (lane == 0) mbar_arrive(&sh.kv_empty[ring.stage]);
-    ring.advance();
-    return true;
+  // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none.
+  auto clean = [&](const Record& rec, int stage, int t) {
+    const int key0 = rec.tile_key(t);
+    if (key0 + kTile <= rec.hi && (key0 >= rec.lo || key0 + kTile <= rec.near)) return;
+    uint8_t* const v = ring_mem + stage * L::kTileBytes;
+    for (int i = lane / 8; i < kTile * L::kHalves; i += 4) {
+      const int k = i / L::kHalves;
+      if (!some_row_sees(rec, key0 + k))
+        *reinterpret_cast<uint4*>(v + (k >> 3) * L::kGroupBytes + (i % L::kHalves) * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
   };
   auto run = [&] {
-    while (records.next(sh, rec)) {
+    while (const Record* const got = records.next(sh)) {
+      const Record rec = *got;   // in registers: the loops below would read it again behind every barrier
       const int n = rec.t1 - rec.t0;
+      const bool pair = rec.pair;
       if (n == 0) continue;
       if (!wait_for(&sh.q_full, q_count & 1, &sh.abort_flag)) return;
       ++q_count;
-      if (rec.pair) {
-        if (!scores(x, n == 1)) return;
-        for (int j = 0; j < n; ++j) {
-          if (!values(rec.t0 + j, j > 0)) return;
-          if (j + 1 < n && !scores(x, j + 2 == n)) return;
+      // The stages come as K 0, V 0, K 1, V 1 ... for a pair, else as K 0, K 1, V 0, K 2, V 1, ... K n - 1, V n - 2, V n - 1.
+      for (int j = 0; j < (pair ? 1 : min(n, 2)); ++j) {
+        if (!wait_stage()) return;
+        tc_fence_after_sync();
+        scores(j, 0);
+        if (pair) scores(1, 1);
+        release(ring.stage);
+        ring.advance();
+      }
+      if (leader && n <= (pair ? 1 : 2)) umma_commit(&sh.q_empty);
+      for (int j = 0; j < n; ++j) {
+        if (!wait_stage()) return;
+        const int v_stage = ring.stage;
+        clean(rec, v_stage, rec.t0 + j);
+        ring.advance();
+        const bool more = pair ? j + 1 < n : j + 2 < n;
+        for (int x = pair ? 0 : j & 1; x <= (pair ? 1 : j & 1); ++x) {
+          if (!values(x, v_stage, pair ? j > 0 : j > 1)) return;
+          if (leader && !pair) umma_commit(&sh.kv_empty[v_stage]);
+          if (!more) {
+            if (leader && pair) umma_commit(&sh.o_full[x]);
+            continue;
+          }
+          if (x == 0 || !pair) {
+            if (!wait_stage()) return;
+            tc_fence_after_sync();
+          }
+          scores(x, pair ? x : 0);
         }
-      } else {
-        // stages: K 0, K 1, V 0, K 2, V 1, ... K n - 1, V n - 2, V n - 1
-        const int mine = (n + 1 - x) / 2;   // tiles of this stream
-        if (x == 0 ? !scores(0, mine == 1) : !pass()) return;
-        if (n > 1 && (x == 1 ? !scores(0, mine == 1) : !pass())) return;
-        if (mine == 0 && leader) umma_commit(&sh.q_empty);
-        for (int j = 0; j < n; ++j) {
-          const bool own = (j & 1) == x;
-          if (own ? !values(rec.t0 + j, j > 1) : !pass()) return;
-          if (j + 2 < n && (own ? !scores(0, j + 4 >= n) : !pass())) return;
+        if (pair) release(v_stage);
+        if (more) {
+          release(ring.stage);
+          if (leader && j + (pair ? 2 : 3) == n) umma_commit(&sh.q_empty);
+          ring.advance();
         }
       }
-      // Only where the stream has tiles: its softmax holds this warp back then. Without, it could complete the barrier twice before
-      // anybody looks.
-      if (leader && (rec.pair || n > x)) umma_commit(&sh.o_full[x]);
+      if (leader && !pair) {
+        umma_commit(&sh.o_full[0]);
+        umma_commit(&sh.o_full[1]);
+      }
     }
   };
   run();
   // whatever ended the loop: nothing of this warp is in flight when it leaves
-  if (leader) umma_commit(&sh.drain[x]);
+  if (leader) umma_commit(&sh.drain);
   int ignored = 0;
-  wait_for(&sh.drain[x], 0, &ignored);
+  wait_for(&sh.drain, 0, &ignored);
 }
 
 template <class E, int D>
@@ -569,41 +647,42 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
   const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
   const uint32_t tmem_s = sh.tmem_base + wg * 128 + lanes, tmem_o = sh.tmem_base + 256 + lanes;
   const int token_in = r / p.group, head_in = r - token_in * p.group;
-  uint32_t s_count = 0, o_count = 0, x_count = 0;
+  uint32_t count = 0, o_count = 0, x_count = 0;   // tiles so far; items; items whose streams were joined
   Records records;
-  Record rec;
   const float scale = p.scale_log2;
-  while (records.next(sh, rec)) {
+  while (const Record* const got = records.next(sh)) {
+    const Record& rec = *got;
     const int n = rec.t1 - rec.t0;
-    const int first = rec.pair ? wg * p.per_stream : 0;                       // first token of the stream in the item
+    const bool pair = rec.pair;
+    const int first = pair ? wg * p.per_stream : 0;                            // first token of the stream in the item
     const int tokens = min(rec.tokens - first, p.per_stream);
     const bool row_ok = r < tokens * p.group;
     const bool works = quad * 32 < tokens * p.group;                           // warp-uniform
-    const int token = first + token_in, row = rec.row0 + token, head = rec.head * p.group + head_in;
-    const int pos = rec.pos0 + token;
-    const int pos_first = rec.pos0 + first, pos_last = pos_first + tokens - 1;
+    // first keys of the tiles that all rows of the stream see: up to full_hi, from full_lo on or up to full_near
+    const int pos_first = rec.pos0 + first;
+    const int full_hi = min(p.tree ? rec.past : pos_first + 1, rec.there) - kTile;
+    const int full_lo = p.tree ? 0 : static_cast<int>(max(0ll, static_cast<long long>(pos_first + tokens) - p.window));
+    const int full_near = p.tree ? 0 : p.sinks - kTile;
+    const int key_base = rec.t0 * kTile, sinks_end = rec.sink_tiles * kTile, jump = (rec.win_tile0 - rec.sink_tiles) * kTile;
     float m = -INFINITY, l = 0.f;
     bool begun = false;
-    for (int j = rec.pair ? 0 : wg; j < n; j += rec.pair ? 1 : 2) {
-      if (!wait_for(&sh.s_full[wg], s_count & 1, &sh.abort_flag)) return;
-      ++s_count;
+#pragma unroll 1
+    for (int j = pair ? 0 : wg; j < n; j += pair ? 1 : 2) {
+      if (!wait_for(&sh.s_full[wg], count & 1, &sh.abort_flag)) return;
+      ++count;
       tc_fence_after_sync();
       if (!works) {   // no row of this warp exists
         tc_fence_before_sync();
         mbar_arrive(&sh.p_full[wg]);
         continue;
       }
-      const int key0 = rec.tile_key(rec.t0 + j);
-      bool full;
-      uint32_t seen[4];
-      if (p.tree) full = key0 + kTile <= min(rec.past, rec.there);
-      else
-        full = key0 + kTile - 1 <= pos_first && key0 + kTile <= rec.there &&
-               (static_cast<long long>(key0) > static_cast<long long>(pos_last) - p.window || key0 + kTile <= p.sinks);
+      int key0 = key_base + j * kTile;
+      if (key0 >= sinks_end) key0 += jump;
+      const bool full = key0 <= full_hi && (key0 >= full_lo || key0 <= full_near);
+      uint32_t seen[4];   // what the row sees of the tile
       if (!full) {
-        // what the row sees of the tile
         if (p.tree) {
-          const int32_t* const words = p.tree + static_cast<size_t>(row_ok ? row : rec.row0) * p.words;
+          const int32_t* const words = p.tree + static_cast<size_t>(rec.row0 + (row_ok ? first + token_in : 0)) * p.words;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int d = key0 + 32 * c - rec.past;   // the drafted token of the first column
@@ -612,6 +691,7 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
             seen[c] = (__funnelshift_r(a, b, s) | bits_of(0, -d)) & bits_of(0, rec.there - key0 - 32 * c);
           }
         } else {
+          const int pos = pos_first + token_in;
           const int hi = max(0, min(min(pos + 1, rec.there) - key0, kTile));
           const int lo = static_cast<int>(max(0ll, min(static_cast<long long>(pos) - p.window + 1 - key0, static_cast<long long>(kTile))));
           const int near = static_cast<int>(min(max(0ll, static_cast<long long>(p.sinks) - key0), static_cast<long long>(hi)));
@@ -619,6 +699,7 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
           for (int c = 0; c < 4; ++c) seen[c] = bits_of(lo - 32 * c, hi - 32 * c) | bits_of(0, near - 32 * c);
         }
       }
+      // The parts of a row one after the other through the same code: straight-line code for all 128 columns is bound by its fetch.
       float mx = -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < kTile; c += 64) {
@@ -632,8 +713,8 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
         }
         float top[4] = {mx, mx, mx, mx};
 #pragma unroll
-        for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
-        mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int i = 0; i < 64; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        mx = max3(fmaxf(top[0], top[1]), top[2], top[3]);
       }
       mx *= scale;
       // The point that a row's exponentials refer to moves when its maximum has grown past it by more than kSlack: weights stay
@@ -645,13 +726,13 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
         if (__any_sync(0xffffffffu, mx > m && row_ok)) {
           const float alpha = mx > m ? exp2_approx(m - mx) : 1.f;
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32(tmem_o + wg * 128 + c, o);
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld_32x16(tmem_o + wg * 128 + c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            store_tmem_32(tmem_o + wg * 128 + c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            store_tmem_16(tmem_o + wg * 128 + c, o);
           }
           l *= alpha;
           m = mx;
@@ -659,35 +740,30 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
       }
       begun = true;
       const float shift = m == -INFINITY ? 0.f : -m;
-      float sum[2] = {0.f, 0.f};
+      Pair sum = 0ull;
 #pragma unroll 1
       for (int c = 0; c < kTile; c += 32) {
-        uint32_t v[32];
+        uint32_t v[32], w[16];
         tmem_ld_32x32(tmem_s + c, v);
         tmem_ld_wait();
         if (!full) hide<32>(v, c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3]));
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float a = exp2_approx(fmaf(__uint_as_float(v[i]), scale, shift)), b = exp2_approx(fmaf(__uint_as_float(v[i + 1]), scale, shift));
-          sum[0] += a;
-          sum[1] += b;
-          v[i / 2] = Half2<E>::pack(a, b);
-        }
-        store_tmem_16(tmem_s + c / 2, v);
+        weigh<E>(v, scale, shift, sum, w);
+        store_tmem_16(tmem_s + c / 2, w);
       }
-      l += sum[0] + sum[1];
+      const float2 sums = parts_of(sum);
+      l += sums.x + sums.y;
       store_tmem_wait();
       tc_fence_before_sync();
       mbar_arrive(&sh.p_full[wg]);
     }
-    if (n > (rec.pair ? 0 : wg)) {   // the stream has tiles
+    if (n > 0) {
       if (!wait_for(&sh.o_full[wg], o_count & 1, &sh.abort_flag)) return;
       ++o_count;
       tc_fence_after_sync();
     }
     // Rows of the item: of a pair both streams have their own; else the streams' results are joined, each group storing half of
     // the columns.
-    E* const out = static_cast<E*>(p.out) + row * p.out_row + head * p.out_head;
+    E* const out = static_cast<E*>(p.out) + (rec.row0 + first + token_in) * p.out_row + (rec.head * p.group + head_in) * p.out_head;
     const size_t ws_row = rec.slot < 0 ? 0 : static_cast<size_t>(rec.slot) * kSlotRows + (rec.pair ? wg * kTile : 0) + r;
     float wa = 1.f, wb = 0.f, total = l, ref = m;
     int c0 = 0, c1 = D, other = 0;
@@ -760,19 +836,19 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     sh.abort_flag = 0;
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&sh.kv_full[i], 1);
-      mbar_init(&sh.kv_empty[i], 2);   // both streams' products
+      mbar_init(&sh.kv_empty[i], 1);
     }
     for (int i = 0; i < kRecords; ++i) {
       mbar_init(&sh.rec_full[i], 1);
-      mbar_init(&sh.rec_empty[i], 11);   // loads, products, queries and eight warps of softmax
+      mbar_init(&sh.rec_empty[i], 10);   // loads, products and eight warps of softmax
     }
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_empty, 2);
+    mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 128);
       mbar_init(&sh.o_full[i], 1);
-      mbar_init(&sh.drain[i], 1);
     }
     mbar_init(&sh.x_full, 256);
     mbar_init(&sh.x_done, 256);
@@ -835,8 +911,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
   if (warp < 4) {
     if (mine) {
       if (warp == 0) produce<D>(p, sh, ring_mem);
+      else if (warp == 1) multiply<E, D>(p, sh, smem, ring_mem);
       else if (warp == 2) schedule<D>(p, sh, smem);
-      else multiply<E, D>(p, sh, smem, ring_mem, warp >> 1);
     }
   } else {
     if (mine) softmax<E, D>(p, sh, (warp - 4) >> 2);

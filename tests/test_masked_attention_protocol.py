@@ -1,5 +1,5 @@
-"""Host model of the masked attention kernel's barriers (csrc/masked_attention.cu): the loading warp, the scheduling warp, a warp
-of products and a group of softmax threads for each stream, with loads and products that finish at any later time, run in random
+"""Host model of the masked attention kernel's barriers (csrc/masked_attention.cu): the loading warp, the scheduling warp, the warp of
+products and a group of softmax threads for each stream, with loads and products that finish at any later time, run in random
 interleavings over random lists of items. No wait may be left, no barrier may complete a phase twice before its waiters have seen
 it (a wait knows only the parity), and no buffer may be written while a reader is left."""
 import random
@@ -29,27 +29,27 @@ class World:
     def __init__(self, items, seed):
         self.items, self.rng = items, random.Random(seed)
         b = Barrier
-        self.kv_full, self.kv_empty = [b(1) for _ in range(STAGES)], [b(2) for _ in range(STAGES)]
-        self.rec_full, self.rec_empty = [b(1) for _ in range(RECORDS)], [b(5) for _ in range(RECORDS)]   # a group reads as one here
-        self.q_full, self.q_empty = b(1), b(2)
-        self.s_full, self.p_full, self.o_full = [b(1), b(1)], [b(1), b(1)], [b(1), b(1)]
+        self.kv_full, self.kv_empty = [b(1) for _ in range(STAGES)], [b(1) for _ in range(STAGES)]
+        self.rec_full, self.rec_empty = [b(1) for _ in range(RECORDS)], [b(4) for _ in range(RECORDS)]   # a group reads as one here
+        self.q_full, self.q_empty = b(1), b(1)
+        self.s_full, self.p_full, self.o_full = ([b(1), b(1)] for _ in range(3))
         self.x_full, self.x_done = b(2), b(2)
         self.q, self.stage, self.s, self.o = None, [None] * STAGES, [None, None], [None, None]
         self.pending = []              # loads, finished in any order
-        self.queue = [[], []]          # of a products warp, finished in order
+        self.queue = []                # products, finished in order
         self.out = {}
 
     def read_records(self):
         n = 0
         while True:
+            if n:
+                self.rec_empty[(n - 1) % RECORDS].arrive()
+                yield None
             yield self.rec_full[n % RECORDS], n // RECORDS
-            item = n if n < len(self.items) else None
-            self.rec_empty[n % RECORDS].arrive()
-            yield None
-            if item is None:
+            if n == len(self.items):
                 return
             n += 1
-            yield ("item", item)
+            yield ("item", n - 1)
 
     def role(self, body):
         """Runs body(item), a generator of waits, for each record."""
@@ -112,50 +112,31 @@ class World:
             self.pending.append(land)
             yield None
 
-    def multiply(self, x):
-        use, q_count, p_count = [0], [0], [0]
+    def multiply(self):
+        use, q_count, p_count = [0], [0], [0, 0]
+        enqueue = lambda *ops: self.queue.extend(ops)   # noqa: E731
 
-        def enqueue(*ops):
-            self.queue[x].extend(ops)
+        def stage():
+            return use[0] % STAGES, (self.kv_full[use[0] % STAGES], use[0] // STAGES)
 
-        def next_stage():
-            u = use[0]
-            use[0] += 1
-            return u % STAGES, (self.kv_full[u % STAGES], u // STAGES)
-
-        def scores(i, j, last):
-            st, wait = next_stage()
-            yield wait
-
+        def scores(x, i, j, st):
             def product():
-                assert self.stage[st] == (i, "K", j) and self.q == i and (self.s[x] is None or self.s[x][0] == "spent"), (self.stage[st], self.q, self.s[x])
+                assert self.stage[st] == (i, "K", j) and self.q == i and self.s[x] in (None, "spent"), (self.stage[st], self.q, self.s[x])
                 self.s[x] = ("S", i, j)
 
-            enqueue(product, self.s_full[x].arrive, self.kv_empty[st].arrive)
-            if last:
-                enqueue(self.q_empty.arrive)
-            yield None
+            enqueue(product, self.s_full[x].arrive)
 
-        def values(i, j, first):
-            st, wait = next_stage()
-            yield wait
-            yield self.p_full[x], p_count[0]
-            p_count[0] += 1
+        def values(x, i, j, st, first):
+            yield self.p_full[x], p_count[x]
+            p_count[x] += 1
 
             def product():
                 assert self.stage[st] == (i, "V", j) and self.s[x] == ("P", i, j), (self.stage[st], self.s[x])
-                assert self.o[x] is None if first else self.o[x][:2] == (i, "sum"), self.o[x]
-                self.o[x] = (i, "sum", ([] if first else self.o[x][2]) + [j])
-                self.s[x] = ("spent",)
+                assert self.o[x] is None if first else self.o[x][0] == i, self.o[x]
+                self.o[x] = (i, ([] if first else self.o[x][1]) + [j])
+                self.s[x] = "spent"
 
-            enqueue(product, self.kv_empty[st].arrive)
-            yield None
-
-        def skip():
-            st, wait = next_stage()
-            yield wait
-            self.kv_empty[st].arrive()
-            yield None
+            enqueue(product)
 
         def body(i):
             n, pair = self.items[i]
@@ -163,26 +144,45 @@ class World:
                 return
             yield self.q_full, q_count[0]
             q_count[0] += 1
-            if pair:
-                yield from scores(i, 0, n == 1)
-                for j in range(n):
-                    yield from values(i, j, j == 0)
-                    if j + 1 < n:
-                        yield from scores(i, j + 1, j + 2 == n)
-            else:
-                mine = (n + 1 - x) // 2
-                yield from (scores(i, 0, mine == 1) if x == 0 else skip())
-                if n > 1:
-                    yield from (scores(i, 1, mine == 1) if x == 1 else skip())
-                if mine == 0:
-                    enqueue(self.q_empty.arrive)
-                for j in range(n):
-                    own = j % 2 == x
-                    yield from (values(i, j, j < 2) if own else skip())
-                    if j + 2 < n:
-                        yield from (scores(i, j + 2, j + 4 >= n) if own else skip())
-            if pair or n > x:
-                enqueue(self.o_full[x].arrive)
+            for j in range(1 if pair else min(n, 2)):
+                st, wait = stage()
+                yield wait
+                scores(j, i, j, st)
+                if pair:
+                    scores(1, i, j, st)
+                enqueue(self.kv_empty[st].arrive)
+                use[0] += 1
+                yield None
+            if n <= (1 if pair else 2):
+                enqueue(self.q_empty.arrive)
+            for j in range(n):
+                v, wait = stage()
+                yield wait
+                use[0] += 1
+                more = j + (1 if pair else 2) < n
+                for x in ((0, 1) if pair else (j % 2,)):
+                    yield from values(x, i, j, v, j < (1 if pair else 2))
+                    if not pair:
+                        enqueue(self.kv_empty[v].arrive)
+                    if not more:
+                        if pair:
+                            enqueue(self.o_full[x].arrive)
+                        continue
+                    k, wait = stage()
+                    if x == 0 or not pair:
+                        yield wait
+                    scores(x, i, j + (1 if pair else 2), k)
+                    yield None
+                if pair:
+                    enqueue(self.kv_empty[v].arrive)
+                if more:
+                    enqueue(self.kv_empty[k].arrive)
+                    if j + (2 if pair else 3) == n:
+                        enqueue(self.q_empty.arrive)
+                    use[0] += 1
+                yield None
+            if not pair:
+                enqueue(self.o_full[0].arrive, self.o_full[1].arrive)
 
         yield from self.role(body)
 
@@ -191,55 +191,57 @@ class World:
 
         def body(i):
             n, pair = self.items[i]
-            for j in range(0 if pair else x, n, 1 if pair else 2):
+            tiles = list(range(0 if pair else x, n, 1 if pair else 2))
+            for j in tiles:
                 yield self.s_full[x], s_count[0]
                 s_count[0] += 1
                 assert self.s[x] == ("S", i, j)
+                if j != tiles[0]:   # where a maximum has grown the sums so far are rescaled
+                    assert self.o[x] == (i, tiles[:tiles.index(j)])
                 self.s[x] = ("P", i, j)
                 yield None
                 self.p_full[x].arrive()
-            if n > (0 if pair else x):
+            if n:
                 yield self.o_full[x], o_count[0]
                 o_count[0] += 1
             if pair:
                 if n:
-                    assert self.o[x] == (i, "sum", list(range(n)))
-                    self.o[x] = None
+                    assert self.o[x] == (i, tiles)
             else:
                 self.x_full.arrive()
                 yield self.x_full, x_count[0]
                 for y in range(2):
                     if n > y:
-                        assert self.o[y] == (i, "sum", list(range(y, n, 2))), (self.o, i, n)
+                        assert self.o[y] == (i, list(range(y, n, 2))), (self.o, i, n)
                 yield None
                 self.x_done.arrive()
                 yield self.x_done, x_count[0]
                 x_count[0] += 1
-                self.o[x] = None
+            self.o[x] = None
             self.out[i, x] = True
 
         yield from self.role(body)
 
     def run(self):
-        roles = [self.produce(), self.schedule(), self.multiply(0), self.multiply(1), self.softmax(0), self.softmax(1)]
+        roles = [self.produce(), self.schedule(), self.multiply(), self.softmax(0), self.softmax(1)]
         waits = [None] * len(roles)
-        speeds = [self.rng.choice([1, 1, 5, 30]) for _ in range(len(roles) + 3)]
+        speeds = [self.rng.choice([1, 1, 5, 30]) for _ in range(len(roles) + 2)]
         while any(r is not None for r in roles):
             ready = [k for k, r in enumerate(roles) if r is not None and (waits[k] is None or waits[k][0].done(waits[k][1]))]
-            choices = ready + [len(roles)] * bool(self.pending) + [len(roles) + 1 + x for x in range(2) if self.queue[x]]
+            choices = ready + [len(roles)] * bool(self.pending) + [len(roles) + 1] * bool(self.queue)
             assert choices, ("nobody can go on", [w and w[1] for w in waits], self.items)
             k = self.rng.choices(choices, [speeds[c] for c in choices])[0]
             if k == len(roles):
                 self.pending.pop(self.rng.randrange(len(self.pending)))()
             elif k > len(roles):
-                self.queue[k - len(roles) - 1].pop(0)()
+                self.queue.pop(0)()
             else:
                 try:
                     waits[k] = next(roles[k])
                 except StopIteration:
                     roles[k] = None
-        while self.pending or any(self.queue):
-            (self.pending or self.queue[0] or self.queue[1]).pop(0)()
+        while self.pending or self.queue:
+            (self.pending or self.queue).pop(0)()
         assert len(self.out) == 2 * len(self.items)
 
 

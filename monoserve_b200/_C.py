@@ -84,7 +84,7 @@ def _load():
     i64 = ctypes.c_int64
     lib.monofab_masked_attention_ws_bytes.restype = i64
     lib.monofab_masked_attention_ws_bytes.argtypes = [i32]
-    lib.monofab_masked_attention.argtypes = [ctypes.POINTER(MaskedAttentionArgsC), vp]
+    lib.monofab_masked_attention.argtypes = [vp, vp]   # MaskedAttentionArgsC by reference, or packed
     lib.monofab_masked_attention_status.argtypes = [ctypes.POINTER(ctypes.c_int32)]
     lib.monofab_qk_rope.argtypes = [vp, i64, vp, vp, vp, i32, vp, vp, vp, i64, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, f32, vp]
     lib.monofab_page_copy.argtypes = [vp, i32, vp, vp, i32, i32, i64, vp, vp]

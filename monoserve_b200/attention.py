@@ -8,7 +8,9 @@ query tokens, key range); long items are split over key ranges for load balance 
 merged by a second small kernel.
 """
 import ctypes
+import functools
 import math
+import struct
 
 import torch
 
@@ -143,66 +145,87 @@ def fabric_tiles(items, merge, args_ptr, kind=K_ATTN_PREFILL):
 # ------------------------------------------------------------------ windows and sinks, trees of drafted tokens
 
 _HALVES = (torch.bfloat16, torch.float16)
+_masked_args = struct.Struct("10Q5q12if4x")   # monofab_masked_attention_args of include/monofab.h
+
+
+# The current stream's handle of a device, without the object that torch.cuda.current_stream makes of it (4 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _no(what):
+    raise ValueError("monofab: " + what)
 
 
 def _refuse(ok, what):
-    if not ok:
-        raise ValueError("monofab: " + what)
+    ok or _no(what)
+
+
+@functools.lru_cache(maxsize=None)
+def _masked_ws_bytes(device_index, head_dim):
+    n = _C.lib.monofab_masked_attention_ws_bytes(head_dim)
+    if n < 0:
+        _C.check(n)
+    return n
 
 
 def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window, sinks, tree, scale, out, stream, status):
-    _refuse(q.dim() == 3 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape,
-            "q is [tokens, hq, head_dim], the caches are [pages, page_size, hkv, head_dim]")
-    T, hq, D = q.shape
-    n_pages, page, hkv, Dk = k_cache.shape
-    _refuse(D == Dk and D in (64, 128), f"head_dim must be 64 or 128 in q and the caches, not {D} and {Dk}")
-    _refuse(q.dtype in _HALVES and k_cache.dtype == q.dtype and v_cache.dtype == q.dtype, "q and the caches are bf16 or fp16, all the same")
-    _refuse(hkv >= 1 and hq >= 1 and hq % hkv == 0 and hq // hkv <= 128, f"hq={hq} must be a multiple of hkv={hkv}, at most 128 times")
-    _refuse(page in (8, 16, 32, 64, 128), f"page_size={page} must be 8, 16, 32, 64 or 128")
-    _refuse(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
-    _refuse(block_table.dim() == 2 and q_start.dim() == 1 and kv_len.dim() == 1, "block_table is [requests, pages], q_start and kv_len are vectors")
+    shape, cache = q.shape, k_cache.shape
+    len(shape) == 3 and len(cache) == 4 and v_cache.shape == cache or \
+        _no("q is [tokens, hq, head_dim], the caches are [pages, page_size, hkv, head_dim]")
+    T, hq, D = shape
+    n_pages, page, hkv, Dk = cache
+    D == Dk and D in (64, 128) or _no(f"head_dim must be 64 or 128 in q and the caches, not {D} and {Dk}")
+    dtype = q.dtype
+    dtype in _HALVES and k_cache.dtype == dtype and v_cache.dtype == dtype or _no("q and the caches are bf16 or fp16, all the same")
+    hkv >= 1 and hq >= 1 and hq % hkv == 0 and hq // hkv <= 128 or _no(f"hq={hq} must be a multiple of hkv={hkv}, at most 128 times")
+    page in (8, 16, 32, 64, 128) or _no(f"page_size={page} must be 8, 16, 32, 64 or 128")
+    k_cache.is_contiguous() and v_cache.is_contiguous() or _no("the caches must be contiguous")
+    tables = block_table.shape
+    len(tables) == 2 and q_start.dim() == 1 and kv_len.dim() == 1 or _no("block_table is [requests, pages], q_start and kv_len are vectors")
     R = kv_len.shape[0]
-    _refuse(block_table.shape[0] == R and q_start.shape[0] == R + 1, f"{R} requests: block_table needs as many rows, q_start one more entry")
+    tables[0] == R and q_start.shape[0] == R + 1 or _no(f"{R} requests: block_table needs as many rows, q_start one more entry")
     small = (block_table, q_start, kv_len) if tree is None else (block_table, q_start, kv_len, tree)
-    _refuse(all(t.dtype == torch.int32 and t.is_contiguous() for t in small), "block_table, q_start, kv_len and tree are contiguous int32")
-    if tree is None:
-        _refuse(1 <= window < 1 << 31 and 0 <= sinks < 1 << 31, f"window={window} must be positive, sinks={sinks} not negative")
-        words = 0
-    else:
-        _refuse(tree.dim() == 2 and tree.shape[0] == T and (tree.shape[1] >= 1 or T == 0), "tree is [tokens, words]")
-        words = tree.shape[1]
-    scale = D ** -0.5 if scale is None else float(scale)
-    _refuse(0.0 < scale < math.inf, "the scale must be positive and finite")
-    if out is not None:
-        _refuse(out.shape == q.shape and out.dtype == q.dtype, "out has the shape and type of q")
-    def strides(t):   # of rows and heads; of a single one it may be anything
-        return t.stride(0) if T > 1 else hq * D, t.stride(1) if hq > 1 else D
-
-    for t in (q,) if out is None else (q, out):
-        (q_row, q_head), last = strides(t), t.stride(2)
-        _refuse(T == 0 or (last == 1 and q_row % 8 == 0 and q_head % 8 == 0 and q_row > 0 and q_head > 0 and t.data_ptr() % 16 == 0),
-                "the heads of q and out must be contiguous and start at multiples of 16 bytes")
     device = q.device
-    _refuse(q.is_cuda and all(t.device == device for t in (k_cache, v_cache, *small)) and (out is None or out.device == device) and
-            (status is None or status.device == device), "all tensors must be on one CUDA device")
-    _refuse(status is None or (status.dtype == torch.int32 and status.numel() >= 1), "status is int32")
-    with torch.cuda.device(device):
-        st = stream if stream is not None else torch.cuda.current_stream()
-        with torch.cuda.stream(st):   # what is allocated here belongs to the stream of the call
-            if out is None:
-                out = torch.empty((T, hq, D), dtype=q.dtype, device=device)
-            if T == 0 or R == 0:
-                return out
-            ws_bytes = _C.lib.monofab_masked_attention_ws_bytes(D)
-            if ws_bytes < 0:
-                _C.check(ws_bytes)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-        a = _C.MaskedAttentionArgsC(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
-            None if tree is None else tree.data_ptr(), ws.data_ptr(), None if status is None else status.data_ptr(),
-            *strides(q), *strides(out), ws_bytes, T, R, hq, hkv, D, page, n_pages, block_table.shape[1], words,
-            0 if tree is not None else window, 0 if tree is not None else sinks, int(q.dtype == torch.float16), scale, 0)
-        _C.check(_C.lib.monofab_masked_attention(ctypes.byref(a), ctypes.c_void_p(st.cuda_stream)))
+    for t in small:
+        t.dtype == torch.int32 and t.is_contiguous() or _no("block_table, q_start, kv_len and tree are contiguous int32")
+    if tree is None:
+        1 <= window < 1 << 31 and 0 <= sinks < 1 << 31 or _no(f"window={window} must be positive, sinks={sinks} not negative")
+        words = tree_at = 0
+    else:
+        window = sinks = 0
+        tree.dim() == 2 and tree.shape[0] == T and (tree.shape[1] >= 1 or T == 0) or _no("tree is [tokens, words]")
+        words, tree_at = tree.shape[1], tree.data_ptr()
+    scale = D ** -0.5 if scale is None else float(scale)
+    0.0 < scale < math.inf or _no("the scale must be positive and finite")
+    out is None or (out.shape == shape and out.dtype == dtype) or _no("out has the shape and type of q")
+
+    def rows_and_heads(t):   # their strides; that of a single one may be anything
+        row, head, last = t.stride()
+        row, head = row if T > 1 else hq * D, head if hq > 1 else D
+        T == 0 or (last == 1 and (row | head) % 8 == 0 and row > 0 and head > 0 and t.data_ptr() % 16 == 0) or \
+            _no("the heads of q and out must be contiguous and start at multiples of 16 bytes")
+        return row, head
+
+    q_strides = rows_and_heads(q)
+    out_strides = (hq * D, D) if out is None else rows_and_heads(out)
+    q.is_cuda and k_cache.device == device and v_cache.device == device and all([t.device == device for t in small]) and \
+        (out is None or out.device == device) and (status is None or status.device == device) or _no("all tensors must be on one CUDA device")
+    status is None or (status.dtype == torch.int32 and status.numel() >= 1) or _no("status is int32")
+    if stream is not None or torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
+            return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window, sinks, tree, scale, out, None, status)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+    if T == 0 or R == 0:
+        return out
+    ws_bytes = _masked_ws_bytes(device.index, D)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    args = _masked_args.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), q_start.data_ptr(),
+                             kv_len.data_ptr(), tree_at, ws.data_ptr(), 0 if status is None else status.data_ptr(), *q_strides, *out_strides, ws_bytes,
+                             T, R, hq, hkv, D, page, n_pages, tables[1], words, window, sinks, dtype == torch.float16, scale)
+    rc = _C.lib.monofab_masked_attention(args, _raw_stream(device.index))
+    if rc:
+        _C.check(rc)
     return out
 
 

@@ -5,17 +5,11 @@ The caches are those of the attention (monoserve_b200/attention.py): [pages, pag
 tensor per layer; page 0 is the sink that unused block-table entries point at (monoserve_b200/engine.py:PagePool).  A
 slot is page * page_size + row in the page.  Like every launch, these wait for a resident fabric to stop.
 """
-import ctypes
-
 import torch
 
 from monoserve_b200 import _C
-from monoserve_b200.attention import _HALVES, _refuse
+from monoserve_b200.attention import _HALVES, _no, _raw_stream, _refuse
 from monoserve_b200.engine import PagePool
-
-
-def _stream_of(stream):
-    return ctypes.c_void_p((stream if stream is not None else torch.cuda.current_stream()).cuda_stream)
 
 
 def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, q_out=None, stream=None):
@@ -28,38 +22,46 @@ def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k
     (2 d, 2 d + 1) if `interleaved`, are turned by the row of the table of its position (outside the table: the nearest
     row).  32-bit arithmetic, one rounding.  Slots outside the cache store nothing: -1 for padding.  q_out [T, hq, D] may be the q
     heads of qkv themselves (qkv.view(T, -1, D)[:, :hq])."""
-    _refuse(qkv.dim() == 2 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "qkv is [T, heads * D], the caches are [pages, page_size, hkv, D]")
-    T = qkv.shape[0]
-    n_pages, page, hkv, D = k_cache.shape
-    _refuse(D in (64, 128, 256), f"head_dim must be 64, 128 or 256, not {D}")
-    _refuse(hq >= 1 and qkv.shape[1] == (hq + 2 * hkv) * D, f"qkv has {qkv.shape[1]} columns, not those of {hq} + 2 * {hkv} heads of {D}")
-    _refuse(qkv.dtype in _HALVES and k_cache.dtype == qkv.dtype and v_cache.dtype == qkv.dtype, "qkv and the caches are bf16 or fp16, all the same")
-    _refuse(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
-    _refuse(n_pages * page < 1 << 31, "the caches have more slots than int32 can name")
-    _refuse(all(t.dim() == 1 and t.shape[0] == T and t.dtype == torch.int32 and t.is_contiguous() for t in (positions, slots)), "positions and slots are int32 [T]")
-    _refuse(cos_sin.dim() == 3 and cos_sin.shape[2] == 2 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous(), "cos_sin is fp32 [max_pos, rot / 2, 2]")
-    rot = 2 * cos_sin.shape[1]
-    _refuse(cos_sin.shape[0] >= 1 and rot % 8 == 0 and rot <= D, f"rot={rot} must be a multiple of 8 up to {D}")
+    cache, dtype, device = k_cache.shape, qkv.dtype, qkv.device
+    qkv.dim() == 2 and len(cache) == 4 and v_cache.shape == cache or _no("qkv is [T, heads * D], the caches are [pages, page_size, hkv, D]")
+    T, columns = qkv.shape
+    n_pages, page, hkv, D = cache
+    D in (64, 128, 256) or _no(f"head_dim must be 64, 128 or 256, not {D}")
+    hq >= 1 and columns == (hq + 2 * hkv) * D or _no(f"qkv has {columns} columns, not those of {hq} + 2 * {hkv} heads of {D}")
+    dtype in _HALVES and k_cache.dtype == dtype and v_cache.dtype == dtype or _no("qkv and the caches are bf16 or fp16, all the same")
+    k_cache.is_contiguous() and v_cache.is_contiguous() or _no("the caches must be contiguous")
+    n_pages * page < 1 << 31 or _no("the caches have more slots than int32 can name")
+    for t in (positions, slots):
+        t.shape == (T,) and t.dtype == torch.int32 and t.is_contiguous() or _no("positions and slots are int32 [T]")
+    table = cos_sin.shape
+    len(table) == 3 and table[2] == 2 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() or _no("cos_sin is fp32 [max_pos, rot / 2, 2]")
+    rot = 2 * table[1]
+    table[0] >= 1 and rot % 8 == 0 and rot <= D or _no(f"rot={rot} must be a multiple of 8 up to {D}")
     norms = [w for w in (q_norm, k_norm) if w is not None]
-    _refuse(all(w.shape == (D,) and w.dtype == qkv.dtype and w.is_contiguous() for w in norms), "q_norm and k_norm are [D] in the type of qkv")
-    _refuse(eps >= 0, "eps must not be negative")
-    _refuse(T == 0 or (qkv.stride(1) == 1 and qkv.stride(0) % 4 == 0 and qkv.stride(0) >= qkv.shape[1] * (T > 1)), "rows of qkv must be contiguous and start at multiples of 8 bytes")
+    for w in norms:
+        w.shape == (D,) and w.dtype == dtype and w.is_contiguous() or _no("q_norm and k_norm are [D] in the type of qkv")
+    eps >= 0 or _no("eps must not be negative")
+    ld, step = qkv.stride()
+    T == 0 or (step == 1 and ld % 4 == 0 and ld >= columns * (T > 1)) or _no("rows of qkv must be contiguous and start at multiples of 8 bytes")
+    tensors = [k_cache, v_cache, positions, slots, cos_sin, *norms]
     if q_out is not None:
-        _refuse(q_out.shape == (T, hq, D) and q_out.dtype == qkv.dtype and q_out.stride(2) == 1 and (hq == 1 or q_out.stride(1) == D) and
-                q_out.stride(0) % 4 == 0 and (T <= 1 or q_out.stride(0) >= hq * D), "q_out is [T, hq, D] with contiguous rows that start at multiples of 8 bytes")
-    device = qkv.device
-    _refuse(qkv.is_cuda and all(t.device == device for t in (k_cache, v_cache, positions, slots, cos_sin, *norms, *(() if q_out is None else (q_out,)))),
-            "all tensors must be on one CUDA device")
-    with torch.cuda.device(device):
-        st = stream if stream is not None else torch.cuda.current_stream()
-        if q_out is None:
-            with torch.cuda.stream(st):
-                q_out = torch.empty((T, hq, D), dtype=qkv.dtype, device=device)
-        _C.check(_C.lib.monofab_qk_rope(
-            qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
-            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), q_out.data_ptr(), q_out.stride(0),
-            k_cache.data_ptr(), v_cache.data_ptr(), n_pages * page, T, hq, hkv, D, rot, int(bool(interleaved)), int(qkv.dtype == torch.float16),
-            float(eps), ctypes.c_void_p(st.cuda_stream)))
+        row, head, last = q_out.stride()
+        q_out.shape == (T, hq, D) and q_out.dtype == dtype and last == 1 and (hq == 1 or head == D) and row % 4 == 0 and \
+            (T <= 1 or row >= hq * D) or _no("q_out is [T, hq, D] with contiguous rows that start at multiples of 8 bytes")
+        tensors.append(q_out)
+    qkv.is_cuda and all([t.device == device for t in tensors]) or _no("all tensors must be on one CUDA device")
+    if stream is not None or torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
+            return qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm, k_norm, eps, interleaved, q_out)
+    if q_out is None:
+        q_out = torch.empty((T, hq, D), dtype=dtype, device=device)
+        row = hq * D
+    rc = _C.lib.monofab_qk_rope(
+        qkv.data_ptr(), ld, positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), table[0], None if q_norm is None else q_norm.data_ptr(),
+        None if k_norm is None else k_norm.data_ptr(), q_out.data_ptr(), row, k_cache.data_ptr(), v_cache.data_ptr(), n_pages * page, T, hq, hkv, D,
+        rot, int(bool(interleaved)), int(dtype == torch.float16), eps, _raw_stream(device.index))
+    if rc:
+        _C.check(rc)
     return q_out
 
 
@@ -144,45 +146,59 @@ class CachePages:
         self.tensors, self.device = tensors, t0.device
         self._table = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64).to(self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._at, self._status_at = self._table.data_ptr(), self.status.data_ptr()
         torch.cuda.current_stream(self.device).synchronize()   # both are there for calls on any stream
 
     def _indexes(self, name, t, *shape):
-        if not isinstance(t, torch.Tensor):
-            t = torch.tensor(t, dtype=torch.int32).reshape(shape).to(self.device)
-        _refuse(t.dtype == torch.int32 and t.is_contiguous() and t.device == self.device and t.dim() == len(shape) and
-                all(s in (-1, n) for s, n in zip(shape, t.shape)), f"{name} is int32 on the device of the cache, of shape {list(shape)}")
-        return t
+        at = t.shape
+        t.dtype == torch.int32 and t.is_contiguous() and t.device == self.device and len(at) == len(shape) or \
+            _no(f"{name} is int32 on the device of the cache, of shape {list(shape)}")
+        for s, n in zip(shape, at):
+            s in (-1, n) or _no(f"{name} is int32 on the device of the cache, of shape {list(shape)}")
+        return at
+
+    def _elsewhere(self, stream):
+        return stream is not None or torch.cuda.current_device() != self.device.index
 
     def copy(self, src, dst, stream=None):
         """Page dst[i] takes what page src[i] holds, in all tensors.  src, dst: int32 tensors on the device, or host lists.  One page
         may go to many, but a destination may be no other pair's source or destination: lists are refused, of tensors such
         pairs (and pages that do not exist) are left out, which check() tells."""
+        if self._elsewhere(stream):
+            with torch.cuda.device(self.device), torch.cuda.stream(stream):
+                return self.copy(src, dst)
         if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
             src, dst = list(src), list(dst)
-            _refuse(len(src) == len(dst) and all(0 <= p < self.n_pages for p in src + dst), "src and dst are as many page numbers of the cache")
+            len(src) == len(dst) and all(0 <= p < self.n_pages for p in src + dst) or _no("src and dst are as many page numbers of the cache")
             pairs = [(s, d) for s, d in zip(src, dst) if s != d]
             src, dst = [s for s, _ in pairs], [d for _, d in pairs]
-            _refuse(len(set(dst)) == len(dst) and not set(dst) & set(src), "a destination is another pair's source or destination")
-        with torch.cuda.device(self.device), torch.cuda.stream(stream):
-            src = self._indexes("src", src, -1)
-            dst = self._indexes("dst", dst, src.shape[0])
-            _refuse(src.shape[0] <= 65535, "at most 65535 pages a call")
-            _C.check(_C.lib.monofab_page_copy(self._table.data_ptr(), len(self.tensors), src.data_ptr(), dst.data_ptr(), src.shape[0], self.n_pages,
-                                              self.page_size * self.row_bytes, self.status.data_ptr(), _stream_of(stream)))
+            len(set(dst)) == len(dst) and not set(dst) & set(src) or _no("a destination is another pair's source or destination")
+            src, dst = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
+        n, = self._indexes("src", src, -1)
+        self._indexes("dst", dst, n)
+        n <= 65535 or _no("at most 65535 pages a call")
+        rc = _C.lib.monofab_page_copy(self._at, len(self.tensors), src.data_ptr(), dst.data_ptr(), n, self.n_pages, self.page_size * self.row_bytes,
+                                      self._status_at, _raw_stream(self.device.index))
+        if rc:
+            _C.check(rc)
 
     def accept(self, block_table, base, path, count, stream=None):
         """The rows of accepted drafts move to the places behind their sequence, in all tensors: of request r, row base[r] + path[r, i]
         to row base[r] + i for i < count[r], as they were before the call.  block_table int32 [requests, stride], base and
         count int32 [requests], path int32 [requests, most <= 2048], on the device.  Rows in places that do not exist stay,
         which check() tells.  Requests must not share the pages of these rows."""
-        block_table = self._indexes("block_table", block_table, -1, -1)
-        R = block_table.shape[0]
-        base, count, path = self._indexes("base", base, R), self._indexes("count", count, R), self._indexes("path", path, R, -1)
-        _refuse(path.shape[1] <= 2048 and R <= 65535 and block_table.shape[1] >= 1, "at most 2048 rows of a path, 65535 requests")
-        with torch.cuda.device(self.device):
-            _C.check(_C.lib.monofab_accept_rows(self._table.data_ptr(), len(self.tensors), block_table.data_ptr(), block_table.shape[1], base.data_ptr(),
-                                                path.data_ptr(), count.data_ptr(), R, path.shape[1], self.page_size, self.n_pages, self.row_bytes,
-                                                self.status.data_ptr(), _stream_of(stream)))
+        if self._elsewhere(stream):
+            with torch.cuda.device(self.device), torch.cuda.stream(stream):
+                return self.accept(block_table, base, path, count)
+        R, width = self._indexes("block_table", block_table, -1, -1)
+        self._indexes("base", base, R)
+        self._indexes("count", count, R)
+        _, most = self._indexes("path", path, R, -1)
+        most <= 2048 and R <= 65535 and width >= 1 or _no("at most 2048 rows of a path, 65535 requests")
+        rc = _C.lib.monofab_accept_rows(self._at, len(self.tensors), block_table.data_ptr(), width, base.data_ptr(), path.data_ptr(), count.data_ptr(), R,
+                                        most, self.page_size, self.n_pages, self.row_bytes, self._status_at, _raw_stream(self.device.index))
+        if rc:
+            _C.check(rc)
 
     def check(self):
         """Raises if a copy or an accept since the last check left something out.  Waits for the device."""

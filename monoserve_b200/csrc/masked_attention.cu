@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kernels.h"
 #include "masked_attention.h"
@@ -23,8 +24,10 @@ namespace {
 constexpr int kTile = 128;          // keys of a tile, rows of a stream
 constexpr int kThreads = 384;
 constexpr int kRecords = 4;
-constexpr int kItemCost = 2;        // what an item costs beyond its tiles, in tiles
-constexpr int kMinCost = 4;         // of a CTA's share
+// What work costs, in tiles of an item whose streams take alternate ones (2000 cycles): a tile of a pair, an item beyond its tiles, and the
+// least share of a CTA.
+constexpr int kPairCost = 2, kItemCost = 2, kMinCost = 2;
+static_assert(kMinCost >= kPairCost, "every share that begins inside an item has a tile of it");
 constexpr int kSlotRows = 2 * kTile;
 constexpr int kMaxRequests = 16384;
 constexpr unsigned long long kWaitNs = 2000000000ull;
@@ -78,6 +81,8 @@ __device__ __forceinline__ int blocks_of(const Params& p, int rows) { return (ro
 struct Span {
   int tokens, pos0, lo, hi, near, sink_tiles, win_tile0, win_tiles;
   __device__ __forceinline__ int tiles() const { return sink_tiles + win_tiles; }
+  __device__ __forceinline__ int tile_cost(const Params& p) const { return tokens > p.per_stream ? kPairCost : 1; }
+  __device__ __forceinline__ int cost(const Params& p) const { return tiles() * tile_cost(p) + kItemCost; }
 };
 __device__ __forceinline__ Span span_of(const Params& p, const Request& q, int block) {
   Span s;
@@ -293,11 +298,12 @@ __device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
   return (0xffffffffu >> (32 - (hi - lo))) << lo;
 }
 
-// Scores whose bit is not set are as low as can be.
-template <int N>
+// Of 32 scores, those whose bit is not set become as low as can be. The border of a window or of the past lies in one or two of a
+// tile's four chunks.
 __device__ __forceinline__ void hide(uint32_t* v, uint32_t seen) {
+  if (__all_sync(0xffffffffu, seen == 0xffffffffu)) return;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = seen >> i & 1u ? v[i] : 0xff800000u;
+  for (int i = 0; i < 32; ++i) v[i] = seen >> i & 1u ? v[i] : 0xff800000u;
 }
 
 // ---------------------------------------------------------------------------------------------------- the shares
@@ -306,7 +312,7 @@ __device__ __forceinline__ void hide(uint32_t* v, uint32_t seen) {
 __device__ __forceinline__ long long request_cost(const Params& p, const Request& q, int lane, int lanes) {
   long long sum = 0;
   const int n = blocks_of(p, q.rows);
-  for (int b = lane; b < n; b += lanes) sum += span_of(p, q, b).tiles() + kItemCost;
+  for (int b = lane; b < n; b += lanes) sum += span_of(p, q, b).cost(p);
   for (int bit = lanes / 2; bit >= 1; bit >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
   return sum * p.hkv;
 }
@@ -330,7 +336,7 @@ __device__ Place place_of(const Params& p, const long long* prefix, long long to
   const int blocks = blocks_of(p, q.rows);
   int cost = 0;
   for (int b0 = 0; b0 < blocks; b0 += 32) {   // 32 blocks at a time
-    const int mine = b0 + lane < blocks ? span_of(p, q, b0 + lane).tiles() + kItemCost : 0;
+    const int mine = b0 + lane < blocks ? span_of(p, q, b0 + lane).cost(p) : 0;
     long long sum = static_cast<long long>(mine) * p.hkv;
     for (int d = 1; d < 32; d <<= 1) {
       const long long up = __shfl_up_sync(0xffffffffu, sum, d);
@@ -349,9 +355,9 @@ __device__ Place place_of(const Params& p, const long long* prefix, long long to
   at.h = static_cast<int>(rest / cost);
   const int off = static_cast<int>(rest - static_cast<long long>(at.h) * cost);
   const long long near = total / shares / 16;
-  if (off <= kItemCost || off <= near) return at;
+  if (off <= near) return at;
   if (cost - off > near) {
-    at.t = off - kItemCost;
+    at.t = max(0, off - kItemCost) / span_of(p, q, at.b).tile_cost(p);
     return at;
   }
   if (++at.h == p.hkv) {
@@ -560,15 +566,15 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
     umma_commit(&sh.s_full[x]);
   };
   auto values = [&](int x, int stage, bool accumulate) {   // O[x] (+)= P[x] V
-    if (!wait_for(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag)) return false;
-    ++p_count[x];
-    tc_fence_after_sync();
     const uint32_t v = (smem_u32(ring_mem) + stage * L::kTileBytes) >> 4 | 64u << 16;
+    if (!wait_for(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag)) return false;
+    tc_fence_after_sync();
     if (leader) {
 #pragma unroll
       for (int i = 0; i < kTile / 16; ++i)
         umma_tmem_a(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, smem_desc(v + i * (L::kGroupBytes / 8), L::kGroupBytes), idesc_o, accumulate || i != 0);
     }
+    ++p_count[x];
     return true;
   };
   // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none.
@@ -628,9 +634,11 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
           ring.advance();
         }
       }
+      // Only of streams that have tiles: their softmax holds this warp back. Without, the barrier could be completed twice before
+      // its waiters look.
       if (leader && !pair) {
         umma_commit(&sh.o_full[0]);
-        umma_commit(&sh.o_full[1]);
+        if (n > 1) umma_commit(&sh.o_full[1]);
       }
     }
   };
@@ -639,6 +647,32 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
   if (leader) umma_commit(&sh.drain);
   int ignored = 0;
   wait_for(&sh.drain, 0, &ignored);
+}
+
+// 64 bytes of each lane's row, at `to` (NULL: of none). Four lanes exchange 16-byte pieces, so that they store 64 bytes of one row side
+// by side: 32 rows' pieces in one instruction, each in another line, take four times as long.
+__device__ __forceinline__ void store_lines(uint32_t (&w)[16], void* to) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1) {   // transposes 4 x 4 pieces
+    const bool hi = lane & bit;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & bit) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t &a = w[4 * i + k], &b = w[4 * (i | bit) + k];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, hi ? a : b, bit);
+        if (hi) a = got;
+        else b = got;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {   // w[4 i ..]: of the group's row i
+    uint4* const row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), (lane & 28) + i));
+    if (row) row[lane & 3] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
 }
 
 template <class E, int D>
@@ -708,8 +742,8 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
         tmem_ld_32x32(tmem_s + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
         tmem_ld_wait();
         if (!full) {
-          hide<32>(&v[0], c ? seen[2] : seen[0]);
-          hide<32>(&v[32], c ? seen[3] : seen[1]);
+          hide(&v[0], c ? seen[2] : seen[0]);
+          hide(&v[32], c ? seen[3] : seen[1]);
         }
         float top[4] = {mx, mx, mx, mx};
 #pragma unroll
@@ -746,7 +780,7 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
         uint32_t v[32], w[16];
         tmem_ld_32x32(tmem_s + c, v);
         tmem_ld_wait();
-        if (!full) hide<32>(v, c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3]));
+        if (!full) hide(v, c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3]));
         weigh<E>(v, scale, shift, sum, w);
         store_tmem_16(tmem_s + c / 2, w);
       }
@@ -756,7 +790,7 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
       tc_fence_before_sync();
       mbar_arrive(&sh.p_full[wg]);
     }
-    if (n > 0) {
+    if (n > (pair ? 0 : wg)) {   // the stream has tiles
       if (!wait_for(&sh.o_full[wg], o_count & 1, &sh.abort_flag)) return;
       ++o_count;
       tc_fence_after_sync();
@@ -799,18 +833,20 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
           f[i] = n > 0 ? __uint_as_float(a[i]) * wa : 0.f;
           if (other && n > 1) f[i] += __uint_as_float(b[i]) * wb;
         }
-        if (row_ok) {
-          if (rec.slot >= 0) {
-            float4* const to = reinterpret_cast<float4*>(p.ws_o + ws_row * D + c);
+        if (rec.slot >= 0) {
+          float* const to = row_ok ? p.ws_o + ws_row * D + c : nullptr;
+          uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-          } else {
-            uint4* const to = reinterpret_cast<uint4*>(out + c);
+          for (int g = 0; g < 2; ++g) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              to[i] = make_uint4(Half2<E>::pack(f[8 * i] * inv, f[8 * i + 1] * inv), Half2<E>::pack(f[8 * i + 2] * inv, f[8 * i + 3] * inv),
-                                 Half2<E>::pack(f[8 * i + 4] * inv, f[8 * i + 5] * inv), Half2<E>::pack(f[8 * i + 6] * inv, f[8 * i + 7] * inv));
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(f[16 * g + i]);
+            store_lines(w, to ? to + 16 * g : nullptr);
           }
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = Half2<E>::pack(f[2 * i] * inv, f[2 * i + 1] * inv);
+          store_lines(w, row_ok ? out + c : nullptr);
         }
         __syncwarp();
       }
@@ -953,17 +989,19 @@ __global__ void __launch_bounds__(256) masked_join_kernel(const __grid_constant_
     for (int q = lane; q < parts; q += 32) top = fmaxf(top, p.ws_ml[slot(q)].x);
     for (int bit = 16; bit; bit >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, bit));
     if (top == -INFINITY) top = 0.f;
-    float sum = 0.f, o[D / 32];
+    constexpr int kOwn = D / 32;   // columns of a lane
+    using Piece = std::conditional_t<kOwn == 4, float4, float2>;
+    float sum = 0.f, o[kOwn];
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) o[d] = 0.f;
+    for (int d = 0; d < kOwn; ++d) o[d] = 0.f;
 #pragma unroll 4
     for (int q = 0; q < parts; ++q) {
       const float2 ml = p.ws_ml[slot(q)];
       const float w = exp2_approx(ml.x - top);
-      const float* const from = p.ws_o + slot(q) * D + lane * (D / 32);
+      const Piece piece = reinterpret_cast<const Piece*>(p.ws_o + slot(q) * D)[lane];
       sum += ml.y * w;
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) o[d] += from[d] * w;
+      for (int d = 0; d < kOwn; ++d) o[d] += reinterpret_cast<const float*>(&piece)[d] * w;
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     E* const out = static_cast<E*>(p.out) + (rows.x + token) * p.out_row + (item.w * p.group + head) * p.out_head + lane * (D / 32);
@@ -993,7 +1031,7 @@ cudaError_t launch(const Params& p, const Grid& g, cudaStream_t stream) {
     return cudaFuncSetAttribute(masked_attention_kernel<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kSmem);
   });
   if (e == cudaSuccess) e = launch_chained(masked_attention_kernel<E, D>, dim3(g.ctas), dim3(kThreads), Layout<D>::kSmem, stream, p);
-  if (e == cudaSuccess && g.ctas > 1) e = launch_chained(masked_join_kernel<E, D>, dim3(g.ctas - 1, 4), dim3(256), 0, stream, p, g.ctas);
+  if (e == cudaSuccess && g.ctas > 1) e = launch_chained(masked_join_kernel<E, D>, dim3(g.ctas - 1, 16), dim3(256), 0, stream, p, g.ctas);
   return e;
 }
 

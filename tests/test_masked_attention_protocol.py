@@ -182,7 +182,7 @@ class World:
                     use[0] += 1
                 yield None
             if not pair:
-                enqueue(self.o_full[0].arrive, self.o_full[1].arrive)
+                enqueue(*[self.o_full[x].arrive for x in range(min(n, 2))])
 
         yield from self.role(body)
 
@@ -201,7 +201,7 @@ class World:
                 self.s[x] = ("P", i, j)
                 yield None
                 self.p_full[x].arrive()
-            if n:
+            if tiles:
                 yield self.o_full[x], o_count[0]
                 o_count[0] += 1
             if pair:

@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "moe_layer.h"
@@ -214,12 +215,17 @@ struct AcceptParams {
   int n_tensors, requests, most, bt_stride, page, n_pages;
   int lanes;           // 16-byte pieces of a row that a block moves, a power of two
   int pieces;          // of a row
+  int per_block;       // tensors of a block
 };
 
-constexpr int kAcceptThreads = 256, kAcceptRows = 8;   // rows a thread holds
+constexpr int kAcceptThreads = 256, kAcceptRows = 8;   // rows a thread holds at most
 
-// Block (slice of a row, tensor, request): every row that moves is read before the first is written, so a path may lead
+// Block (slice of a row, group of tensors, request): every row that moves is read before the first is written, so a path may lead
 // anywhere among the drafts, whatever it overwrites. The slice is as wide as lets the block's threads hold all rows.
+// What bounds it is the chain count, path, table, row: it is gone through once for a group of tensors, and the next
+// tensor's rows are on their way while the last one's are written. (64 requests, 96 tensors, 5 rows of 1 KB each: a block for each
+// tensor 42 us, see the table of times for what it takes now.)
+template <int kRows>
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptParams p) {
   chain_release();
   chain_wait();
@@ -228,38 +234,61 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_con
   const long long base = p.base[r];
   const int piece = blockIdx.x * p.lanes + threadIdx.x % p.lanes;
   const int row0 = threadIdx.x / p.lanes, step = kAcceptThreads / p.lanes;
-  char* const tensor = reinterpret_cast<char*>(p.tensors[blockIdx.y]);
   const int32_t* const table = p.block_table + static_cast<long long>(r) * p.bt_stride;
+  const long long there = static_cast<long long>(p.bt_stride) * p.page;
   bool bad = false;
-  auto address = [&](long long at) -> char* {
-    if (at < 0 || at >= static_cast<long long>(p.bt_stride) * p.page) return nullptr;
-    const int page = table[at / p.page];
-    if (page < 0 || page >= p.n_pages) return nullptr;
-    return tensor + ((static_cast<long long>(page) * p.page + at % p.page) * p.pieces + piece) * 16;
-  };
-  uint4 v[kAcceptRows];
-  char* to[kAcceptRows];
+  long long from[kRows], to[kRows];   // in a tensor; from < 0: nothing to move
 #pragma unroll
-  for (int i = 0; i < kAcceptRows; ++i) {
+  for (int i = 0; i < kRows; ++i) {
     const int row = row0 + i * step;
-    to[i] = nullptr;
+    from[i] = -1;
     if (row >= n) continue;
-    const int from_row = p.path[static_cast<long long>(r) * p.most + row];
-    const char* const from = from_row < 0 ? nullptr : address(base + from_row);
-    char* const dst = address(base + row);
-    if (!from || !dst) {
+    const int taken = p.path[static_cast<long long>(r) * p.most + row];
+    const long long src = base + taken, dst = base + row;
+    if (taken < 0 || base < 0 || src >= there || dst >= there) {
       bad = true;
       continue;
     }
-    if (from == dst || piece >= p.pieces) continue;
-    v[i] = *reinterpret_cast<const uint4*>(from);
-    to[i] = dst;
+    const uint32_t a = static_cast<uint32_t>(src), b = static_cast<uint32_t>(dst), page = p.page;
+    const int pa = table[a / page], pb = table[b / page];
+    if (pa < 0 || pa >= p.n_pages || pb < 0 || pb >= p.n_pages) {
+      bad = true;
+      continue;
+    }
+    if (taken == row || piece >= p.pieces) continue;
+    from[i] = ((static_cast<long long>(pa) * page + a % page) * p.pieces + piece) * 16;
+    to[i] = ((static_cast<long long>(pb) * page + b % page) * p.pieces + piece) * 16;
   }
-  if (bad) atomicOr(p.status, kErrBadArgs);
-  __syncthreads();
+  if (bad && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(p.status, kErrBadArgs);
+  const int t0 = blockIdx.y * p.per_block, t1 = min(t0 + p.per_block, p.n_tensors);
+  uint4 v[kRows];
+  auto load = [&](int t, uint4(&into)[kRows]) {
+    const char* const tensor = reinterpret_cast<const char*>(p.tensors[t]);
 #pragma unroll
-  for (int i = 0; i < kAcceptRows; ++i)
-    if (to[i]) *reinterpret_cast<uint4*>(to[i]) = v[i];
+    for (int i = 0; i < kRows; ++i)
+      if (from[i] >= 0) into[i] = *reinterpret_cast<const uint4*>(tensor + from[i]);
+  };
+  load(t0, v);
+  for (int t = t0; t < t1; ++t) {
+    uint4 next[kRows];
+    if (t + 1 < t1) load(t + 1, next);
+    __syncthreads();   // all rows of this tensor have been read
+    char* const tensor = reinterpret_cast<char*>(p.tensors[t]);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      if (from[i] >= 0) *reinterpret_cast<uint4*>(tensor + to[i]) = v[i];
+      v[i] = next[i];
+    }
+  }
+}
+
+// Blocks that the current device runs at a time with `each` on an SM.
+int sm_blocks(int* blocks, int each) {
+  int device = 0, sms = 0;
+  MF_CUDA(cudaGetDevice(&device));
+  MF_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  *blocks = sms * each;
+  return MONOFAB_OK;
 }
 
 }  // namespace
@@ -366,7 +395,14 @@ extern "C" int monofab_accept_rows(const uint64_t* tensors, int n_tensors, const
   p.pieces = static_cast<int>(row_bytes / 16);
   p.lanes = 1;
   while (2 * p.lanes <= kAcceptThreads && 2 * p.lanes * most <= kAcceptThreads * kAcceptRows && p.lanes < p.pieces) p.lanes *= 2;
-  MF_CUDA(launch_chained(accept_kernel, dim3((p.pieces + p.lanes - 1) / p.lanes, n_tensors, requests), dim3(kAcceptThreads), 0,
-                         static_cast<cudaStream_t>(stream), p));
+  const int slices = (p.pieces + p.lanes - 1) / p.lanes, rows = (most * p.lanes + kAcceptThreads - 1) / kAcceptThreads;
+  // as many tensors a block as leave every SM its blocks
+  int blocks = 0;
+  if (int e = sm_blocks(&blocks, 8)) return e;
+  const long long all = static_cast<long long>(slices) * n_tensors * requests;
+  p.per_block = static_cast<int>(std::max(1ll, std::min(16ll, all / blocks)));
+  const dim3 grid(slices, (n_tensors + p.per_block - 1) / p.per_block, requests);
+  auto go = [&](auto kernel) { return launch_chained(kernel, grid, dim3(kAcceptThreads), 0, static_cast<cudaStream_t>(stream), p); };
+  MF_CUDA(rows <= 2 ? go(accept_kernel<2>) : rows <= 4 ? go(accept_kernel<4>) : go(accept_kernel<kAcceptRows>));
   return MONOFAB_OK;
 }

@@ -1,5 +1,33 @@
 // Attention over a paged cache with a window and sinks, or with a tree of drafted tokens behind the past, on tcgen05 /
-// TMEM / TMA.
+// TMEM / TMA (monofab_masked_attention in monofab.h says what is computed).
+//
+// o_i = sum_j p_ij v_j / sum_j p_ij over the keys j that row i sees, p_ij = 2^(c s_ij - m_i), s = q k, c = scale log2(e), in one
+// pass over the keys in tiles of 128. m_i is a reference that all of a row's weights share: the first maximum, moved only when a later
+// one passes it by more than 2^8, and then the sums so far are scaled. Scores, sums and outputs are in 32 bits; a weight is rounded
+// once, to the type of V, for the product.
+//
+//   * An item is (request, block of query tokens, KV head); a row of the matrix products is a (token, query head of the group) pair,
+//     so a K or V tile is read once for all of them. A CTA has two streams of 128 rows, each with scores S (128 columns of TMEM), the
+//     weights P in the place of the scores that they come from (64 columns, the A operand of P V) and an accumulator O (D
+//     columns): 512 columns for D = 128. In an item of more rows than one stream takes (a pair) the streams have a block of rows each
+//     and share the tiles; else they take alternate tiles of the same rows and are joined at the end.
+//   * Warps: 0 loads K and V through a ring of 32 or 16 KB stages; 1 issues the products; 2 hands out items and loads queries; 4 - 7
+//     and 8 - 11 are the streams' softmax, a thread a row. One warp issues both streams' products: it keeps them a step apart, so
+//     that one's products run under the other's softmax. (A warp for each: their products run into each other, both streams wait at the
+//     same time; window prompts 177 -> 187 us.)
+//   * The work is shared out on the device, from lengths that are read there: tiles and items have a cost (below), every
+//     CTA takes an equal part of its sum, and items that a border cuts leave 32-bit rows and (reference, sum) in a workspace,
+//     which a second kernel joins in order: the same bits every time. A border near an item's begin is moved there.
+//   * A tile that all rows of a stream see goes without masks; else a row has the tile's keys as bits: the ranges of the window
+//     and the sinks, or the past and the tree's bits, shifted. Pages that no row of the item sees are not loaded, and values that
+//     none sees are zeroed in shared memory, so that nothing there can reach a sum.
+//
+// What bounds it (B200, clocks as they come): contexts of single tokens HBM, 5.5 TB/s of K and V (128 sequences, 844 MB: 153 us);
+// prompts and large trees the softmax: a pair's tile takes 3400 cycles, of which its products take 2048 and the exponentials of both
+// streams 2048 of the special-function units, one stream's rows 2050 from S to P and 1350 from P to the next S. Measured and dropped: a row
+// of S in registers (straight-line code for 128 columns is bound by its fetch: long trees 448 -> 505 us), sixteen warps of softmax
+// (500 -> 530), half tiles with two score buffers a stream (467; its scores cost half as much again), weights handed over in two parts (no
+// change), the next columns' TMEM loads ahead of the weights (469 -> 500).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -250,3 +250,29 @@ def test_scale_and_large_scores():
     tol = tolerance(ref, weighted, BF, 1100) + 1.8e-3 * weighted
     err = (out.double().cpu() - ref).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+def test_as_many_requests_as_a_call_takes():
+    R = 16384
+    rows, past = [1] * R, [r % 3 for r in range(R)]
+    batch = make(rows, past, 1, 1, 64, 8, BF, seed=21)
+    check(run_sliding(batch, 2, 0), batch, sliding_masks(batch, 2, 0))
+
+
+def test_a_status_word_of_ones_own():
+    from monoserve_b200.attention import attention_status, sliding_attention
+    batch = on_gpu(*make([3], [200], 8, 2, 64, 16, FP, seed=22))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want = sliding_attention(*batch, 50)
+    assert torch.equal(sliding_attention(*batch, 50, status=status), want)
+    assert status.item() == 0 and attention_status() == 0
+    q, *rest = batch
+    assert sliding_attention(q[:0], *rest[:3], torch.zeros(2, dtype=torch.int32, device="cuda"), rest[4], 50).shape == (0, 8, 64)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert sliding_attention(q[:0], *rest[:2], rest[2][:0], none.new_zeros(1), none, 50).shape == (0, 8, 64)
+
+
+def test_groups_of_128_and_wide_kv_heads():
+    for hq, hkv, rows in ((128, 1, [1, 3]), (256, 2, [2, 1]), (40, 40, [200, 1]), (24, 8, [90, 43])):
+        batch = make(rows, [300, 129], hq, hkv, 64, 32, BF, seed=hq)
+        check(run_sliding(batch, 200, 7), batch, sliding_masks(batch, 200, 7))

@@ -81,6 +81,7 @@ def test_attention_entry_point_refuses():
     refused(b"16 bytes", out_row=1025)
     refused(b"2^30", bt_stride=1 << 28)
     refused(b"workspace", ws_bytes=0)
+    refused(b"at most 16384", requests=16385)
     assert _C.lib.monofab_masked_attention(None, None) == -1
     a = _C.MaskedAttentionArgsC(**{**good, "tokens": 0})
     assert _C.lib.monofab_masked_attention(ctypes.byref(a), None) == 0   # nothing to do

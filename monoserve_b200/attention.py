@@ -176,7 +176,7 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     n_pages, page, hkv, Dk = cache
     D == Dk and D in (64, 128) or _no(f"head_dim must be 64 or 128 in q and the caches, not {D} and {Dk}")
     dtype = q.dtype
-    dtype in _HALVES and k_cache.dtype == dtype and v_cache.dtype == dtype or _no("q and the caches are bf16 or fp16, all the same")
+    dtype in _HALVES and k_cache.dtype is dtype and v_cache.dtype is dtype or _no("q and the caches are bf16 or fp16, all the same")
     hkv >= 1 and hq >= 1 and hq % hkv == 0 and hq // hkv <= 128 or _no(f"hq={hq} must be a multiple of hkv={hkv}, at most 128 times")
     page in (8, 16, 32, 64, 128) or _no(f"page_size={page} must be 8, 16, 32, 64 or 128")
     k_cache.is_contiguous() and v_cache.is_contiguous() or _no("the caches must be contiguous")
@@ -185,9 +185,10 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     R = kv_len.shape[0]
     tables[0] == R and q_start.shape[0] == R + 1 or _no(f"{R} requests: block_table needs as many rows, q_start one more entry")
     small = (block_table, q_start, kv_len) if tree is None else (block_table, q_start, kv_len, tree)
-    device = q.device
+    index, here = q.get_device(), True
     for t in small:
-        t.dtype == torch.int32 and t.is_contiguous() or _no("block_table, q_start, kv_len and tree are contiguous int32")
+        t.dtype is torch.int32 and t.is_contiguous() or _no("block_table, q_start, kv_len and tree are contiguous int32")
+        here = here and t.get_device() == index
     if tree is None:
         1 <= window < 1 << 31 and 0 <= sinks < 1 << 31 or _no(f"window={window} must be positive, sinks={sinks} not negative")
         words = tree_at = 0
@@ -199,31 +200,31 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     0.0 < scale < math.inf or _no("the scale must be positive and finite")
     out is None or (out.shape == shape and out.dtype == dtype) or _no("out has the shape and type of q")
 
-    def rows_and_heads(t):   # their strides; that of a single one may be anything
+    out_strides = hq * D, D
+    for t in (q,) if out is None else (out, q):   # strides of rows and heads; that of a single one may be anything
         row, head, last = t.stride()
-        row, head = row if T > 1 else hq * D, head if hq > 1 else D
+        if T <= 1 or hq == 1:
+            row, head = row if T > 1 else hq * D, head if hq > 1 else D
         T == 0 or (last == 1 and (row | head) % 8 == 0 and row > 0 and head > 0 and t.data_ptr() % 16 == 0) or \
             _no("the heads of q and out must be contiguous and start at multiples of 16 bytes")
-        return row, head
-
-    q_strides = rows_and_heads(q)
-    out_strides = (hq * D, D) if out is None else rows_and_heads(out)
-    q.is_cuda and k_cache.device == device and v_cache.device == device and all([t.device == device for t in small]) and \
-        (out is None or out.device == device) and (status is None or status.device == device) or _no("all tensors must be on one CUDA device")
+        if t is out:
+            out_strides = row, head
+    index >= 0 and here and k_cache.get_device() == index and v_cache.get_device() == index and \
+        (out is None or out.get_device() == index) and (status is None or status.get_device() == index) or _no("all tensors must be on one CUDA device")
     status is None or (status.dtype == torch.int32 and status.numel() >= 1) or _no("status is int32")
-    if stream is not None or torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
+    if stream is not None or torch.cuda.current_device() != index:
+        with torch.cuda.device(index), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
             return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window, sinks, tree, scale, out, None, status)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = q.new_empty(shape)
     if T == 0 or R == 0:
         return out
-    ws_bytes = _masked_ws_bytes(device.index, D)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    ws_bytes = _masked_ws_bytes(index, D)
+    ws = block_table.new_empty(ws_bytes >> 2)
     args = _masked_args.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), q_start.data_ptr(),
-                             kv_len.data_ptr(), tree_at, ws.data_ptr(), 0 if status is None else status.data_ptr(), *q_strides, *out_strides, ws_bytes,
-                             T, R, hq, hkv, D, page, n_pages, tables[1], words, window, sinks, dtype == torch.float16, scale)
-    rc = _C.lib.monofab_masked_attention(args, _raw_stream(device.index))
+                             kv_len.data_ptr(), tree_at, ws.data_ptr(), 0 if status is None else status.data_ptr(), row, head, *out_strides, ws_bytes,
+                             T, R, hq, hkv, D, page, n_pages, tables[1], words, window, sinks, dtype is torch.float16, scale)
+    rc = _C.lib.monofab_masked_attention(args, _raw_stream(index))
     if rc:
         _C.check(rc)
     return out

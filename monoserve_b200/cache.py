@@ -22,13 +22,13 @@ def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k
     (2 d, 2 d + 1) if `interleaved`, are turned by the row of the table of its position (outside the table: the nearest
     row).  32-bit arithmetic, one rounding.  Slots outside the cache store nothing: -1 for padding.  q_out [T, hq, D] may be the q
     heads of qkv themselves (qkv.view(T, -1, D)[:, :hq])."""
-    cache, dtype, device = k_cache.shape, qkv.dtype, qkv.device
+    cache, dtype, index = k_cache.shape, qkv.dtype, qkv.get_device()
     qkv.dim() == 2 and len(cache) == 4 and v_cache.shape == cache or _no("qkv is [T, heads * D], the caches are [pages, page_size, hkv, D]")
     T, columns = qkv.shape
     n_pages, page, hkv, D = cache
     D in (64, 128, 256) or _no(f"head_dim must be 64, 128 or 256, not {D}")
     hq >= 1 and columns == (hq + 2 * hkv) * D or _no(f"qkv has {columns} columns, not those of {hq} + 2 * {hkv} heads of {D}")
-    dtype in _HALVES and k_cache.dtype == dtype and v_cache.dtype == dtype or _no("qkv and the caches are bf16 or fp16, all the same")
+    dtype in _HALVES and k_cache.dtype is dtype and v_cache.dtype is dtype or _no("qkv and the caches are bf16 or fp16, all the same")
     k_cache.is_contiguous() and v_cache.is_contiguous() or _no("the caches must be contiguous")
     n_pages * page < 1 << 31 or _no("the caches have more slots than int32 can name")
     for t in (positions, slots):
@@ -49,17 +49,18 @@ def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k
         q_out.shape == (T, hq, D) and q_out.dtype == dtype and last == 1 and (hq == 1 or head == D) and row % 4 == 0 and \
             (T <= 1 or row >= hq * D) or _no("q_out is [T, hq, D] with contiguous rows that start at multiples of 8 bytes")
         tensors.append(q_out)
-    qkv.is_cuda and all([t.device == device for t in tensors]) or _no("all tensors must be on one CUDA device")
-    if stream is not None or torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
+    for t in tensors:
+        t.get_device() == index and index >= 0 or _no("all tensors must be on one CUDA device")
+    if stream is not None or torch.cuda.current_device() != index:
+        with torch.cuda.device(index), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
             return qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm, k_norm, eps, interleaved, q_out)
     if q_out is None:
-        q_out = torch.empty((T, hq, D), dtype=dtype, device=device)
+        q_out = qkv.new_empty((T, hq, D))
         row = hq * D
     rc = _C.lib.monofab_qk_rope(
         qkv.data_ptr(), ld, positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), table[0], None if q_norm is None else q_norm.data_ptr(),
         None if k_norm is None else k_norm.data_ptr(), q_out.data_ptr(), row, k_cache.data_ptr(), v_cache.data_ptr(), n_pages * page, T, hq, hkv, D,
-        rot, int(bool(interleaved)), int(dtype == torch.float16), eps, _raw_stream(device.index))
+        rot, int(bool(interleaved)), int(dtype == torch.float16), eps, _raw_stream(index))
     if rc:
         _C.check(rc)
     return q_out

@@ -58,6 +58,7 @@ constexpr int kPairCost = 2, kItemCost = 2, kMinCost = 2;
 static_assert(kMinCost >= kPairCost, "every share that begins inside an item has a tile of it");
 constexpr int kSlotRows = 2 * kTile;
 constexpr int kMaxRequests = 16384;
+constexpr int kFewRows = 16, kFewBytes = 2 * kFewRows * 128;   // kFewBytes: weights of such a stream, two times 64 keys of a row in 128 bytes
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr float kSlack = 8.f;
 constexpr int kByFma = 4;           // weights of 32 worked out by multiplications
@@ -145,6 +146,7 @@ struct Record {
   int sink_tiles, win_tile0, t0, t1;
   int slot;     // -1: the whole item, else the workspace slot
   int pair;     // two streams of rows; else the streams take alternate tiles. -1: no more items
+  int few;      // not a pair, and few enough rows to be the columns of the scores (kFewRows)
   __device__ __forceinline__ int tile_key(int t) const { return kTile * (t < sink_tiles ? t : t - sink_tiles + win_tile0); }
 };
 
@@ -159,12 +161,17 @@ struct Layout {
 
 struct Shared {
   uint64_t kv_full[10], kv_empty[10], rec_full[kRecords], rec_empty[kRecords];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], x_full, x_done, drain;
+  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], told[2], x_full, x_done, drain;
   uint32_t tmem_base;
   int abort_flag;
   Place place[2];
   Record rec[kRecords];
-  float2 ml[2][kTile];
+  union {
+    float2 ml[2][kTile];   // (reference, sum) of the streams' rows
+    struct {               // of an item of few rows: of each stream, warp and row, maxima of a tile and sums of the item; references
+      float top[2][4][kFewRows], sum[2][4][kFewRows], m[2][kFewRows];
+    } few;
+  };
 };
 
 // Descriptors: Q rows of 128 bytes a half, halves 16 KB apart; K and V tiles in groups of eight keys, the halves of a group
@@ -205,6 +212,12 @@ __device__ __forceinline__ void store_tmem_16(uint32_t taddr, const uint32_t* r)
       : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void load_tmem_4(uint32_t at, uint32_t (&v)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(at)
+               : "memory");
 }
 __device__ __forceinline__ void store_tmem_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -448,6 +461,7 @@ __device__ void schedule(const Params& p, Shared& sh, uint8_t* q_mem) {
       const int cta = static_cast<int>(blockIdx.x);
       rec.slot = rec.t0 > 0 ? 2 * cta : rec.t1 < tiles ? 2 * cta + 1 : -1;
       rec.pair = s.tokens > p.per_stream;
+      rec.few = D == 128 && s.tokens * p.group <= kFewRows;
       at.t = 0;
       if (same_item(at, end)) at.r = p.requests;   // nothing behind it
       else if (++at.h == p.hkv) {
@@ -618,6 +632,51 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
     fence_proxy_async_smem();
     __syncwarp();
   };
+  // An item of few rows: S^T[x] = K Q^T and O^T[x] (+)= V^T P^T[x]. Apart from the others, whose loop pays for every instruction.
+  auto run_few = [&](const Record& rec, int n) {
+    auto scores_few = [&](int x) {
+      if (!wait_stage()) return false;
+      tc_fence_after_sync();
+      if (leader) {
+        const uint32_t q = smem_u32(q_mem) >> 4, k = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          umma_bf16(tmem + x * 128, smem_desc(k + (i >> 2) * 64 + (i & 3) * 2, L::kGroupBytes), smem_desc(q + (i >> 2) * (kTile * 8) + (i & 3) * 2, 1024),
+                    idesc_of<E>(kFewRows), i != 0);
+        umma_commit(&sh.s_full[x]);
+        umma_commit(&sh.kv_empty[ring.stage]);
+      }
+      ring.advance();
+      return true;
+    };
+    for (int j = 0; j < min(n, 2); ++j)
+      if (!scores_few(j)) return false;
+    for (int j = 0; j < n; ++j) {
+      const int x = j & 1;
+      if (!wait_stage()) return false;
+      clean(rec, ring.stage, rec.t0 + j);
+      if (!wait_for(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag)) return false;
+      ++p_count[x];
+      tc_fence_after_sync();
+      if (leader) {
+        const uint32_t v = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4 | 64u << 16;
+        const uint32_t w = smem_u32(q_mem + L::kTileBytes + x * kFewBytes) >> 4;
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+          umma_bf16(tmem + 256 + x * 128, smem_desc(v + i * (L::kGroupBytes / 8), L::kGroupBytes), smem_desc(w + (i >> 2) * (kFewRows * 8) + (i & 3) * 2, 1024),
+                    idesc_of<E>(kFewRows) | 1u << 15, j > 1 || i != 0);   // V is MN-major
+        umma_commit(&sh.kv_empty[ring.stage]);
+      }
+      ring.advance();
+      if (j + 2 < n && !scores_few(x)) return false;
+    }
+    if (leader) {
+      umma_commit(&sh.q_empty);   // not before: the weights lie where a pair's other queries go
+      umma_commit(&sh.o_full[0]);
+      if (n > 1) umma_commit(&sh.o_full[1]);
+    }
+    return true;
+  };
   auto run = [&] {
     while (const Record* const got = records.next(sh)) {
       const Record rec = *got;   // in registers: the loops below would read it again behind every barrier
@@ -626,6 +685,12 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
       if (n == 0) continue;
       if (!wait_for(&sh.q_full, q_count & 1, &sh.abort_flag)) return;
       ++q_count;
+      if constexpr (D == 128) {
+        if (rec.few) {
+          if (!run_few(rec, n)) return;
+          continue;
+        }
+      }
       // The stages come as K 0, V 0, K 1, V 1 ... for a pair, else as K 0, K 1, V 0, K 2, V 1, ... K n - 1, V n - 2, V n - 1.
       for (int j = 0; j < (pair ? 1 : min(n, 2)); ++j) {
         if (!wait_stage()) return;
@@ -703,17 +768,196 @@ __device__ __forceinline__ void store_lines(uint32_t (&w)[16], void* to) {
   }
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+struct Counts {   // phases of the barriers so far: tiles, items with tiles, joined items, tiles of few rows
+  uint32_t s = 0, o = 0, x = 0, told = 0;
+};
+
+// An item of at most 16 rows: S^T = K Q^T and O^T = V^T P^T, keys and head dims on the 128 lanes and the rows as columns, so that
+// neither the products nor the exponentials are of 128 rows. A thread has a key of each tile. A row's reference is known to all of a
+// stream's threads and held by lane `row`, too; the weights go to shared memory, as the other operand.
+// (128 sequences of single tokens, 844 MB: see the file's head; with 128 rows of which eight are there it drew the card's power limit.)
+template <class E>
+__device__ bool softmax_few(const Params& p, Shared& sh, uint8_t* q_mem, const Record& rec, int wg, Counts& c) {
+  constexpr int D = 128, N = kFewRows;
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, r = quad * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+  const uint32_t tmem_s = sh.tmem_base + wg * 128 + lanes, tmem_o = sh.tmem_base + 256 + lanes;
+  uint8_t* const mine = q_mem + Layout<D>::kTileBytes + wg * kFewBytes + (r >> 6) * (kFewRows * 128) + (r & 7) * 2;   // the key's place in row 0
+  const int chunk = (r & 63) >> 3;
+  const int n = rec.t1 - rec.t0, rows = rec.tokens * p.group;
+  const float scale = p.scale_log2;
+  float m[N], l[N], held = -INFINITY;   // held: the reference of row `lane`
+#pragma unroll
+  for (int i = 0; i < N; ++i) m[i] = l[i] = 0.f;
+  bool begun = false;
+#pragma unroll 1
+  for (int j = wg; j < n; j += 2) {
+    if (!wait_for(&sh.s_full[wg], c.s & 1, &sh.abort_flag)) return false;
+    ++c.s;
+    tc_fence_after_sync();
+    const int key0 = rec.tile_key(rec.t0 + j), key = key0 + r;
+    float s[N];
+    {
+      uint32_t v[N];
+      tmem_ld_32x16(tmem_s, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] = __uint_as_float(v[i]) * scale;
+    }
+    bool full;
+    if (p.tree) full = key0 + kTile <= min(rec.past, rec.there);
+    else full = key0 + kTile <= min(rec.pos0 + 1, rec.there) &&
+                (key0 >= static_cast<long long>(rec.pos0) + rec.tokens - p.window || key0 + kTile <= p.sinks);
+    if (!full) {
+      uint32_t seen = 0;   // the rows that see the key
+      const uint32_t token = (1u << p.group) - 1u;
+      for (int t = 0; t < rec.tokens; ++t) {
+        bool sees = key < rec.there;
+        if (p.tree) {
+          const int d = key - rec.past;
+          if (d >= 0) sees = sees && (d >> 5) < p.words && (p.tree[static_cast<size_t>(rec.row0 + t) * p.words + (d >> 5)] >> (d & 31) & 1);
+        } else {
+          const int pos = rec.pos0 + t;
+          sees = sees && key <= pos && (key > static_cast<long long>(pos) - p.window || key < p.sinks);
+        }
+        if (sees) seen |= token << (t * p.group);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] = seen >> i & 1u ? s[i] : -INFINITY;
+    }
+    float own = -INFINITY;   // the warp's maximum of row `lane`
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float top = warp_max(s[i]);
+      if (lane == i) own = top;
+    }
+    if (lane < N) sh.few.top[wg][quad][lane] = own;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.told[wg]);
+    if (!wait_for(&sh.told[wg], c.told & 1, &sh.abort_flag)) return false;
+    ++c.told;
+    float top = -INFINITY;
+    if (lane < rows) top = fmaxf(fmaxf(sh.few.top[wg][0][lane], sh.few.top[wg][1][lane]), fmaxf(sh.few.top[wg][2][lane], sh.few.top[wg][3][lane]));
+    const bool grows = begun ? top > held + kSlack : true;
+    if (__any_sync(0xffffffffu, lane < rows && grows)) {   // of all four warps alike
+      const float moved = grows ? top : held;
+      if (begun) {   // S of this tile is there, so P V of the stream's tile before it is, too
+        const float alpha = moved > held ? exp2_approx(held - moved) : 1.f;
+        uint32_t o[N];
+        tmem_ld_32x16(tmem_o + wg * 128, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float a = __shfl_sync(0xffffffffu, alpha, i);
+          o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+          l[i] *= a;
+        }
+        store_tmem_16(tmem_o + wg * 128, o);
+        store_tmem_wait();
+      }
+      held = moved;
+      const float shift = held == -INFINITY ? 0.f : held;
+#pragma unroll
+      for (int i = 0; i < N; ++i) m[i] = __shfl_sync(0xffffffffu, shift, i);
+    }
+    begun = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float w = exp2_approx(s[i] - m[i]);
+      l[i] += w;
+      *reinterpret_cast<E*>(mine + i * 128 + ((chunk ^ (i & 7)) << 4)) = static_cast<E>(w);
+    }
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    mbar_arrive(&sh.p_full[wg]);
+  }
+  if (n > wg) {   // the stream has tiles
+    if (!wait_for(&sh.o_full[wg], c.o & 1, &sh.abort_flag)) return false;
+    ++c.o;
+    tc_fence_after_sync();
+  }
+  float sum = 0.f;   // the warp's part of row `lane`'s sum
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float t = l[i];
+#pragma unroll
+    for (int bit = 16; bit; bit >>= 1) t += __shfl_xor_sync(0xffffffffu, t, bit);
+    if (lane == i) sum = t;
+  }
+  if (lane < N) sh.few.sum[wg][quad][lane] = sum;
+  if (quad == 0 && lane < N) sh.few.m[wg][lane] = held;
+  mbar_arrive(&sh.x_full);
+  if (!wait_for(&sh.x_full, c.x & 1, &sh.abort_flag)) return false;
+  tc_fence_after_sync();
+  // of row `lane`: how the streams are joined
+  const int at = min(lane, N - 1);
+  const float ma = sh.few.m[0][at], mb = sh.few.m[1][at], ref = fmaxf(ma, mb), shift = ref == -INFINITY ? 0.f : ref;
+  const float ea = exp2_approx(ma - shift), eb = exp2_approx(mb - shift);
+  float sums[2] = {0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    sums[0] += sh.few.sum[0][q][at];
+    sums[1] += sh.few.sum[1][q][at];
+  }
+  const float total = sums[0] * ea + sums[1] * eb;
+  const float inv = rec.slot >= 0 ? 1.f : total > 0.f ? 1.f / total : 0.f;
+  // where row `lane` goes; the streams' threads store every other row
+  const int token = at / p.group, head = rec.head * p.group + at - token * p.group;
+  unsigned long long to = 0;
+  if (lane < rows)
+    to = rec.slot >= 0 ? reinterpret_cast<unsigned long long>(p.ws_o + (static_cast<size_t>(rec.slot) * kSlotRows + lane) * D)
+                       : reinterpret_cast<unsigned long long>(static_cast<E*>(p.out) + (rec.row0 + token) * p.out_row + head * p.out_head);
+  const float fa = n > 0 ? ea * inv : 0.f, fb = n > 1 ? eb * inv : 0.f;
+#pragma unroll 1
+  for (int c0 = 0; c0 < rows; c0 += 4) {
+    uint32_t a[4], b[4];   // head dim r of four rows, of the two streams
+    if (n > 0) load_tmem_4(tmem_o + c0, a);
+    if (n > 1) load_tmem_4(tmem_o + 128 + c0, b);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float ga = __shfl_sync(0xffffffffu, fa, c0 + i), gb = __shfl_sync(0xffffffffu, fb, c0 + i);
+      const unsigned long long row = __shfl_sync(0xffffffffu, to, c0 + i);
+      if ((i & 1) == wg && row) {
+        float f = n > 0 ? __uint_as_float(a[i]) * ga : 0.f;
+        if (n > 1) f = fmaf(__uint_as_float(b[i]), gb, f);
+        if (rec.slot >= 0) reinterpret_cast<float*>(row)[r] = f;
+        else reinterpret_cast<E*>(row)[r] = static_cast<E>(f);
+      }
+    }
+    __syncwarp();
+  }
+  if (rec.slot >= 0 && quad == 0 && wg == 0 && lane < rows) p.ws_ml[static_cast<size_t>(rec.slot) * kSlotRows + lane] = make_float2(ref, total);
+  tc_fence_before_sync();
+  mbar_arrive(&sh.x_done);
+  if (!wait_for(&sh.x_done, c.x & 1, &sh.abort_flag)) return false;
+  ++c.x;
+  return true;
+}
+
 template <class E, int D>
-__device__ void softmax(const Params& p, Shared& sh, int wg) {
+__device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, r = quad * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
   const uint32_t tmem_s = sh.tmem_base + wg * 128 + lanes, tmem_o = sh.tmem_base + 256 + lanes;
   const int token_in = r / p.group, head_in = r - token_in * p.group;
-  uint32_t count = 0, o_count = 0, x_count = 0;   // tiles so far; items; items whose streams were joined
+  Counts counts;
   Records records;
   const float scale = p.scale_log2;
   while (const Record* const got = records.next(sh)) {
     const Record& rec = *got;
+    if constexpr (D == 128) {
+      if (rec.few) {
+        if (!softmax_few<E>(p, sh, q_mem, rec, wg, counts)) return;
+        continue;
+      }
+    }
     const int n = rec.t1 - rec.t0;
     const bool pair = rec.pair;
     const int first = pair ? wg * p.per_stream : 0;                            // first token of the stream in the item
@@ -730,8 +974,8 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
     bool begun = false;
 #pragma unroll 1
     for (int j = pair ? 0 : wg; j < n; j += pair ? 1 : 2) {
-      if (!wait_for(&sh.s_full[wg], count & 1, &sh.abort_flag)) return;
-      ++count;
+      if (!wait_for(&sh.s_full[wg], counts.s & 1, &sh.abort_flag)) return;
+      ++counts.s;
       tc_fence_after_sync();
       if (!works) {   // no row of this warp exists
         tc_fence_before_sync();
@@ -819,8 +1063,8 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
       mbar_arrive(&sh.p_full[wg]);
     }
     if (n > (pair ? 0 : wg)) {   // the stream has tiles
-      if (!wait_for(&sh.o_full[wg], o_count & 1, &sh.abort_flag)) return;
-      ++o_count;
+      if (!wait_for(&sh.o_full[wg], counts.o & 1, &sh.abort_flag)) return;
+      ++counts.o;
       tc_fence_after_sync();
     }
     // Rows of the item: of a pair both streams have their own; else the streams' results are joined, each group storing half of
@@ -832,7 +1076,7 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
     if (!rec.pair) {
       sh.ml[wg][r] = make_float2(m, l);
       mbar_arrive(&sh.x_full);
-      if (!wait_for(&sh.x_full, x_count & 1, &sh.abort_flag)) return;
+      if (!wait_for(&sh.x_full, counts.x & 1, &sh.abort_flag)) return;
       tc_fence_after_sync();   // the other stream's products are there, too: its threads have waited for them
       const float2 a = sh.ml[0][r], b = sh.ml[1][r];
       ref = fmaxf(a.x, b.x);
@@ -883,8 +1127,8 @@ __device__ void softmax(const Params& p, Shared& sh, int wg) {
     tc_fence_before_sync();
     if (!rec.pair) {   // the accumulators and the exchange are free once both groups have read them
       mbar_arrive(&sh.x_done);
-      if (!wait_for(&sh.x_done, x_count & 1, &sh.abort_flag)) return;
-      ++x_count;
+      if (!wait_for(&sh.x_done, counts.x & 1, &sh.abort_flag)) return;
+      ++counts.x;
     }
   }
 }
@@ -913,6 +1157,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 128);
       mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.told[i], 4);
     }
     mbar_init(&sh.x_full, 256);
     mbar_init(&sh.x_done, 256);
@@ -979,7 +1224,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
       else if (warp == 2) schedule<D>(p, sh, smem);
     }
   } else {
-    if (mine) softmax<E, D>(p, sh, (warp - 4) >> 2);
+    if (mine) softmax<E, D>(p, sh, smem, (warp - 4) >> 2);
   }
   __syncwarp();
   tc_fence_before_sync();

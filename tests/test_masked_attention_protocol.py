@@ -34,6 +34,8 @@ class World:
         self.q_full, self.q_empty = b(1), b(1)
         self.s_full, self.p_full, self.o_full = ([b(1), b(1)] for _ in range(3))
         self.x_full, self.x_done = b(2), b(2)
+        self.told = [b(4), b(4)]       # an item of few rows: the warps of a stream tell each other their maxima
+        self.weights = [None, None]    # of such a stream, where the other queries of a pair go
         self.q, self.stage, self.s, self.o = None, [None] * STAGES, [None, None], [None, None]
         self.pending = []              # loads, finished in any order
         self.queue = []                # products, finished in order
@@ -77,7 +79,7 @@ class World:
             yield None
 
         def body(i):
-            n, pair = self.items[i]
+            n, pair, few = self.items[i]
             if pair:
                 for j in range(n):
                     yield from load((i, "K", j))
@@ -106,6 +108,8 @@ class World:
 
             def land(n=n):
                 self.q = n
+                if self.items[n][1]:
+                    assert self.weights == [None, None], "weights were overwritten"
                 self.q_full.arrive()
 
             self.q = None
@@ -132,6 +136,9 @@ class World:
 
             def product():
                 assert self.stage[st] == (i, "V", j) and self.s[x] == ("P", i, j), (self.stage[st], self.s[x])
+                if self.items[i][2]:
+                    assert self.weights[x] == (i, j)
+                    self.weights[x] = None
                 assert self.o[x] is None if first else self.o[x][0] == i, self.o[x]
                 self.o[x] = (i, ([] if first else self.o[x][1]) + [j])
                 self.s[x] = "spent"
@@ -139,7 +146,7 @@ class World:
             enqueue(product)
 
         def body(i):
-            n, pair = self.items[i]
+            n, pair, few = self.items[i]
             if n == 0:
                 return
             yield self.q_full, q_count[0]
@@ -153,7 +160,7 @@ class World:
                 enqueue(self.kv_empty[st].arrive)
                 use[0] += 1
                 yield None
-            if n <= (1 if pair else 2):
+            if not few and n <= (1 if pair else 2):
                 enqueue(self.q_empty.arrive)
             for j in range(n):
                 v, wait = stage()
@@ -177,20 +184,22 @@ class World:
                     enqueue(self.kv_empty[v].arrive)
                 if more:
                     enqueue(self.kv_empty[k].arrive)
-                    if j + (2 if pair else 3) == n:
+                    if not few and j + (2 if pair else 3) == n:
                         enqueue(self.q_empty.arrive)
                     use[0] += 1
                 yield None
+            if few:
+                enqueue(self.q_empty.arrive)
             if not pair:
                 enqueue(*[self.o_full[x].arrive for x in range(min(n, 2))])
 
         yield from self.role(body)
 
     def softmax(self, x):
-        s_count, o_count, x_count = [0], [0], [0]
+        s_count, o_count, x_count, told = [0], [0], [0], [0]
 
         def body(i):
-            n, pair = self.items[i]
+            n, pair, few = self.items[i]
             tiles = list(range(0 if pair else x, n, 1 if pair else 2))
             for j in tiles:
                 yield self.s_full[x], s_count[0]
@@ -198,6 +207,14 @@ class World:
                 assert self.s[x] == ("S", i, j)
                 if j != tiles[0]:   # where a maximum has grown the sums so far are rescaled
                     assert self.o[x] == (i, tiles[:tiles.index(j)])
+                if few:   # this thread of control is one of the four warps, the others' are taken along
+                    for _ in range(4):
+                        self.told[x].arrive()
+                        yield None
+                    yield self.told[x], told[0]
+                    told[0] += 1
+                    assert self.weights[x] is None and self.q == i
+                    self.weights[x] = (i, j)
                 self.s[x] = ("P", i, j)
                 yield None
                 self.p_full[x].arrive()
@@ -249,5 +266,6 @@ class World:
 def test_random_interleavings(seed):
     rng = random.Random(seed)
     for k in range(12):
-        items = [(rng.choice([0, 1, 1, 2, 3, 5, 8]), rng.random() < rng.choice([0.0, 0.5, 1.0])) for _ in range(rng.randrange(1, 14))]
-        World([(n, pair) for n, pair in items], 1000 * seed + k).run()
+        kinds = rng.choice([["pair"], ["few", "pair"], ["few", "alternate", "pair"], ["few", "alternate"], ["alternate", "pair"]])
+        items = [(rng.choice([0, 1, 1, 2, 3, 5, 8]), rng.choice(kinds)) for _ in range(rng.randrange(1, 14))]
+        World([(n, kind == "pair", kind == "few") for n, kind in items], 1000 * seed + k).run()

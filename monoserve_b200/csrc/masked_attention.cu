@@ -11,6 +11,8 @@
 //     weights P in the place of the scores that they come from (64 columns, the A operand of P V) and an accumulator O (D
 //     columns): 512 columns for D = 128. In an item of more rows than one stream takes (a pair) the streams have a block of rows each
 //     and share the tiles; else they take alternate tiles of the same rows and are joined at the end.
+//   * An item of at most 16 rows (a token and its group) in a batch of such (D = 128) is multiplied the other way round, keys and head
+//     dims as the 128 rows and its rows as 16 columns (softmax_few).
 //   * Warps: 0 loads K and V through a ring of 32 or 16 KB stages; 1 issues the products; 2 hands out items and loads queries; 4 - 7
 //     and 8 - 11 are the streams' softmax, a thread a row. One warp issues both streams' products: it keeps them a step apart, so
 //     that one's products run under the other's softmax. (A warp for each: their products run into each other, both streams wait at the
@@ -22,7 +24,7 @@
 //     and the sinks, or the past and the tree's bits, shifted. Pages that no row of the item sees are not loaded, and values that
 //     none sees are zeroed in shared memory, so that nothing there can reach a sum.
 //
-// What bounds it (B200, clocks as they come): contexts of single tokens HBM, 5.5 TB/s of K and V (128 sequences, 844 MB: 153 us);
+// What bounds it (B200, clocks as they come): contexts of single tokens HBM, 5.6 TB/s of K and V (128 sequences, 843 MB: 151 us);
 // prompts and large trees the softmax: a pair's tile takes 3400 cycles, of which its products take 2048 and the exponentials of both
 // streams 2048 of the special-function units, one stream's rows 2050 from S to P and 1350 from P to the next S. Measured and dropped: a row
 // of S in registers (straight-line code for 128 columns is bound by its fetch: long trees 448 -> 505 us), sixteen warps of softmax
@@ -413,7 +415,7 @@ __device__ Place place_of(const Params& p, const long long* prefix, long long to
 }
 
 // Writes the records of the items from place[0] to place[1], and loads each one's queries once the scores of the one before have read theirs.
-template <int D>
+template <int D, bool kFew>
 __device__ void schedule(const Params& p, Shared& sh, uint8_t* q_mem) {
   using L = Layout<D>;
   const int lane = threadIdx.x & 31;
@@ -461,7 +463,7 @@ __device__ void schedule(const Params& p, Shared& sh, uint8_t* q_mem) {
       const int cta = static_cast<int>(blockIdx.x);
       rec.slot = rec.t0 > 0 ? 2 * cta : rec.t1 < tiles ? 2 * cta + 1 : -1;
       rec.pair = s.tokens > p.per_stream;
-      rec.few = D == 128 && s.tokens * p.group <= kFewRows;
+      rec.few = kFew && s.tokens * p.group <= kFewRows;
       at.t = 0;
       if (same_item(at, end)) at.r = p.requests;   // nothing behind it
       else if (++at.h == p.hkv) {
@@ -584,7 +586,7 @@ __device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
 }
 
 // The products of both streams, by one warp: it keeps them a step apart, so that one stream's products run under the other's softmax.
-template <class E, int D>
+template <class E, int D, bool kFew>
 __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* ring_mem) {
   using L = Layout<D>;
   const int lane = threadIdx.x & 31;
@@ -685,7 +687,7 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
       if (n == 0) continue;
       if (!wait_for(&sh.q_full, q_count & 1, &sh.abort_flag)) return;
       ++q_count;
-      if constexpr (D == 128) {
+      if constexpr (kFew) {
         if (rec.few) {
           if (!run_few(rec, n)) return;
           continue;
@@ -781,7 +783,6 @@ struct Counts {   // phases of the barriers so far: tiles, items with tiles, joi
 // An item of at most 16 rows: S^T = K Q^T and O^T = V^T P^T, keys and head dims on the 128 lanes and the rows as columns, so that
 // neither the products nor the exponentials are of 128 rows. A thread has a key of each tile. A row's reference is known to all of a
 // stream's threads and held by lane `row`, too; the weights go to shared memory, as the other operand.
-// (128 sequences of single tokens, 844 MB: see the file's head; with 128 rows of which eight are there it drew the card's power limit.)
 template <class E>
 __device__ bool softmax_few(const Params& p, Shared& sh, uint8_t* q_mem, const Record& rec, int wg, Counts& c) {
   constexpr int D = 128, N = kFewRows;
@@ -941,7 +942,7 @@ __device__ bool softmax_few(const Params& p, Shared& sh, uint8_t* q_mem, const R
   return true;
 }
 
-template <class E, int D>
+template <class E, int D, bool kFew>
 __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, r = quad * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
@@ -952,7 +953,7 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
   const float scale = p.scale_log2;
   while (const Record* const got = records.next(sh)) {
     const Record& rec = *got;
-    if constexpr (D == 128) {
+    if constexpr (kFew) {
       if (rec.few) {
         if (!softmax_few<E>(p, sh, q_mem, rec, wg, counts)) return;
         continue;
@@ -1133,7 +1134,7 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
   }
 }
 
-template <class E, int D>
+template <class E, int D, bool kFew>
 __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __grid_constant__ Params p) {
   using L = Layout<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -1220,11 +1221,11 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
   if (warp < 4) {
     if (mine) {
       if (warp == 0) produce<D>(p, sh, ring_mem);
-      else if (warp == 1) multiply<E, D>(p, sh, smem, ring_mem);
-      else if (warp == 2) schedule<D>(p, sh, smem);
+      else if (warp == 1) multiply<E, D, kFew>(p, sh, smem, ring_mem);
+      else if (warp == 2) schedule<D, kFew>(p, sh, smem);
     }
   } else {
-    if (mine) softmax<E, D>(p, sh, smem, (warp - 4) >> 2);
+    if (mine) softmax<E, D, kFew>(p, sh, smem, (warp - 4) >> 2);
   }
   __syncwarp();
   tc_fence_before_sync();
@@ -1334,13 +1335,13 @@ Grid grid_of(int head_dim, int sms) {
   return g;
 }
 
-template <class E, int D>
+template <class E, int D, bool kFew = false>
 cudaError_t launch(const Params& p, const Grid& g, cudaStream_t stream) {
   static PerDeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(masked_attention_kernel<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kSmem);
+    return cudaFuncSetAttribute(masked_attention_kernel<E, D, kFew>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kSmem);
   });
-  if (e == cudaSuccess) e = launch_chained(masked_attention_kernel<E, D>, dim3(g.ctas), dim3(kThreads), Layout<D>::kSmem, stream, p);
+  if (e == cudaSuccess) e = launch_chained(masked_attention_kernel<E, D, kFew>, dim3(g.ctas), dim3(kThreads), Layout<D>::kSmem, stream, p);
   if (e == cudaSuccess && g.ctas > 1) e = launch_chained(masked_join_kernel<E, D>, dim3(g.ctas - 1, 8), dim3(256), 0, stream, p, g.ctas);
   return e;
 }
@@ -1434,8 +1435,15 @@ extern "C" int monofab_masked_attention(const monofab_masked_attention_args* a, 
   p.sinks = a->sinks;
   p.scale_log2 = a->scale * 1.44269504088896340736f;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->fp16) MF_CUDA((D == 64 ? launch<__half, 64>(p, g, st) : launch<__half, 128>(p, g, st)));
-  else MF_CUDA((D == 64 ? launch<__nv_bfloat16, 64>(p, g, st) : launch<__nv_bfloat16, 128>(p, g, st)));
+  // Batches of single tokens and the like (by the mean of their rows: what the host knows) take the kernel that also has a form for items
+  // of few rows. 128 single tokens over 843 MB, long runs: 153 us, without the form 177 (at the card's power limit: 128 rows of products
+  // for eight that are there); but its code alone, unused, makes window prompts 157 -> 162.
+  const bool few = static_cast<int64_t>(a->tokens) * group <= static_cast<int64_t>(a->requests) * kFewRows;
+  auto go = [&](auto e) {
+    using E = decltype(e);
+    return D == 64 ? launch<E, 64>(p, g, st) : few ? launch<E, 128, true>(p, g, st) : launch<E, 128>(p, g, st);
+  };
+  MF_CUDA(a->fp16 ? go(__half()) : go(__nv_bfloat16()));
   return MONOFAB_OK;
 }
 

@@ -276,3 +276,41 @@ def test_groups_of_128_and_wide_kv_heads():
     for hq, hkv, rows in ((128, 1, [1, 3]), (256, 2, [2, 1]), (40, 40, [200, 1]), (24, 8, [90, 43])):
         batch = make(rows, [300, 129], hq, hkv, 64, 32, BF, seed=hq)
         check(run_sliding(batch, 200, 7), batch, sliding_masks(batch, 200, 7))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("hq,hkv", [(32, 4), (12, 4), (5, 5), (16, 1), (96, 8)])
+def test_batches_of_few_rows(dtype, hq, hkv):
+    """At most 16 rows of a KV head a request on the mean: those requests' rows are the columns of the products, others among
+    them (of a pair, too) are not. Windows, sinks and trees; every kind of item behind every other."""
+    from monoserve_b200.attention import tree_attention
+    group = hq // hkv
+    few = max(1, 16 // group)
+    rows = [1, few, 0, 1, few, 0, 0, 1, 1, 0, 0, 0, 0, 1]
+    past = [3000, 700, 10, 0, 129, 5, 7, 128, 2048, 0, 0, 1, 2, 60]
+    big = 16 // group * len(rows) - sum(rows)   # as many more as the mean allows
+    if big > 0:
+        rows[9], past[9] = big, 333
+    batch = make(rows, past, hq, hkv, 128, 16, dtype, seed=hq + 31)
+    assert sum(rows) * group <= 16 * len(rows)
+    for window, sinks in ((1 << 30, 0), (100, 3), (129, 140), (1, 0)):
+        check(run_sliding(batch, window, sinks), batch, sliding_masks(batch, window, sinks))
+    for empty in (False, True):
+        tree = random_trees(rows, hq, empty)
+        check(tree_attention(*on_gpu(*batch), tree.cuda()), batch, tree_masks(batch, tree))
+
+
+def test_few_rows_whose_maxima_grow_and_unseen_values():
+    """Maxima that grow from tile to tile, so that sums are rescaled, and NaN in what nobody sees."""
+    q, kc, vc, bt, start, kv = make([1, 1, 1], [3000, 1000, 1], 32, 4, 128, 16, BF, seed=33, fill=float("nan"))
+    ramp = torch.zeros(kc.shape[0])
+    for r, L in enumerate(kv.tolist()):
+        for j in range(-(-L // 16)):
+            ramp[bt[r, j]] = (j + 1) / 128
+    batch = (q.sign(), (kc.sign() * ramp[:, None, None, None]).to(BF), vc, bt, start, kv)
+    out = run_sliding(batch, 1 << 30, 0, scale=1.0)
+    ref, weighted = reference(*batch, sliding_masks(batch, 1 << 30, 0), scale=1.0)
+    # 128 exact products of at most 1.5: their 32-bit sum is off by less than 128 * 2^-24 * 128 * 1.5 = 1.5e-3
+    tol = tolerance(ref, weighted, BF, 3100) + 1.5e-3 * weighted
+    err = (out.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())

@@ -177,10 +177,19 @@ int monofab_masked_attention_status(int32_t* out);
  * q_out (rows ld_out values apart; may be the q heads of qkv themselves), k and v heads to slot (page * page size + row in
  * the page) slots[t] of caches [n_slots][hkv][head_dim]; slots outside [0, n_slots) (padding: -1) store nothing.  Rows
  * stored in one slot in one call leave one or the other's values there.  head_dim 64, 128 or 256; values bf16, or fp16. */
-int monofab_qk_rope(const void* qkv, int64_t ld_qkv, const int32_t* positions, const int32_t* slots, const float* cos_sin,
-                    int max_pos, const void* q_norm, const void* k_norm, void* q_out, int64_t ld_out, void* k_cache,
-                    void* v_cache, int64_t n_slots, int T, int hq, int hkv, int head_dim, int rot, int interleaved, int fp16,
-                    float eps, void* stream);
+typedef struct {
+  const void* qkv;
+  const int32_t* positions;    /* [T] */
+  const int32_t* slots;        /* [T] */
+  const float* cos_sin;
+  const void *q_norm, *k_norm; /* [head_dim], or NULL */
+  void *q_out, *k_cache, *v_cache;
+  int64_t ld_qkv, ld_out, n_slots;
+  int32_t T, hq, hkv, head_dim, rot, max_pos, interleaved, fp16;
+  float eps;
+  int32_t reserved;
+} monofab_qk_rope_args;
+int monofab_qk_rope(const monofab_qk_rope_args* args, void* stream);
 
 /* Page dst[i] takes what page src[i] holds, in all n_tensors cache tensors (device array of addresses, each
  * [n_pages][page_bytes], 16-byte aligned).  A pair whose page numbers lie outside [0, n_pages), whose destination is

@@ -62,6 +62,14 @@ class MaskedAttentionArgsC(ctypes.Structure):
                 [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)])
 
 
+class QkRopeArgsC(ctypes.Structure):
+    """struct monofab_qk_rope_args of include/monofab.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("qkv", "positions", "slots", "cos_sin", "q_norm", "k_norm", "q_out", "k_cache", "v_cache")] +
+                [(n, ctypes.c_int64) for n in ("ld_qkv", "ld_out", "n_slots")] +
+                [(n, ctypes.c_int32) for n in ("T", "hq", "hkv", "head_dim", "rot", "max_pos", "interleaved", "fp16")] +
+                [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing: build it with `python -m monoserve_b200.build` "
@@ -86,7 +94,7 @@ def _load():
     lib.monofab_masked_attention_ws_bytes.argtypes = [i32]
     lib.monofab_masked_attention.argtypes = [vp, vp]   # MaskedAttentionArgsC by reference, or packed
     lib.monofab_masked_attention_status.argtypes = [ctypes.POINTER(ctypes.c_int32)]
-    lib.monofab_qk_rope.argtypes = [vp, i64, vp, vp, vp, i32, vp, vp, vp, i64, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, f32, vp]
+    lib.monofab_qk_rope.argtypes = [vp, vp]             # QkRopeArgsC by reference, or packed
     lib.monofab_page_copy.argtypes = [vp, i32, vp, vp, i32, i32, i64, vp, vp]
     lib.monofab_accept_rows.argtypes = [vp, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i64, vp, vp]
     lib.monofab_combine.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, f32, vp]

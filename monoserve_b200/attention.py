@@ -216,7 +216,7 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
         with torch.cuda.device(index), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
             return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window, sinks, tree, scale, out, None, status)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     if T == 0 or R == 0:
         return out
     ws_bytes = _masked_ws_bytes(index, D)

@@ -5,11 +5,16 @@ The caches are those of the attention (monoserve_b200/attention.py): [pages, pag
 tensor per layer; page 0 is the sink that unused block-table entries point at (monoserve_b200/engine.py:PagePool).  A
 slot is page * page_size + row in the page.  Like every launch, these wait for a resident fabric to stop.
 """
+import struct
+
 import torch
 
 from monoserve_b200 import _C
 from monoserve_b200.attention import _HALVES, _no, _raw_stream, _refuse
 from monoserve_b200.engine import PagePool
+
+
+_rope_args = struct.Struct("9Q3q8if4x")   # monofab_qk_rope_args of include/monofab.h
 
 
 def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, q_out=None, stream=None):
@@ -57,10 +62,10 @@ def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k
     if q_out is None:
         q_out = qkv.new_empty((T, hq, D))
         row = hq * D
-    rc = _C.lib.monofab_qk_rope(
-        qkv.data_ptr(), ld, positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), table[0], None if q_norm is None else q_norm.data_ptr(),
-        None if k_norm is None else k_norm.data_ptr(), q_out.data_ptr(), row, k_cache.data_ptr(), v_cache.data_ptr(), n_pages * page, T, hq, hkv, D,
-        rot, int(bool(interleaved)), int(dtype == torch.float16), eps, _raw_stream(index))
+    args = _rope_args.pack(qkv.data_ptr(), positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
+                           0 if k_norm is None else k_norm.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ld, row,
+                           n_pages * page, T, hq, hkv, D, rot, table[0], bool(interleaved), dtype is torch.float16, eps)
+    rc = _C.lib.monofab_qk_rope(args, _raw_stream(index))
     if rc:
         _C.check(rc)
     return q_out

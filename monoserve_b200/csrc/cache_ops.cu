@@ -318,51 +318,49 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_con
 
 using namespace mf;
 
-extern "C" int monofab_qk_rope(const void* qkv, int64_t ld_qkv, const int32_t* positions, const int32_t* slots,
-                               const float* cos_sin, int max_pos, const void* q_norm, const void* k_norm, void* q_out,
-                               int64_t ld_out, void* k_cache, void* v_cache, int64_t n_slots, int T, int hq, int hkv,
-                               int head_dim, int rot, int interleaved, int fp16, float eps, void* stream) {
+extern "C" int monofab_qk_rope(const monofab_qk_rope_args* a, void* stream) {
+  if (!a) return fail(MONOFAB_EINVAL, "qk_rope: NULL argument");
+  const int T = a->T, hq = a->hq, hkv = a->hkv, D = a->head_dim, rot = a->rot;
   if (T < 0) return fail(MONOFAB_EINVAL, "qk_rope: negative T");
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
-    return fail(MONOFAB_EINVAL, "qk_rope: head_dim=%d must be 64, 128 or 256", head_dim);
+  if (D != 64 && D != 128 && D != 256) return fail(MONOFAB_EINVAL, "qk_rope: head_dim=%d must be 64, 128 or 256", D);
   if (hq < 0 || hkv < 0 || hq + hkv < 1 || hq > (1 << 16) || hkv > (1 << 16)) return fail(MONOFAB_EINVAL, "qk_rope: hq=%d, hkv=%d", hq, hkv);
-  if (rot < 0 || rot > head_dim || rot % 8) return fail(MONOFAB_EINVAL, "qk_rope: rot=%d must be a multiple of 8 up to head_dim", rot);
+  if (rot < 0 || rot > D || rot % 8) return fail(MONOFAB_EINVAL, "qk_rope: rot=%d must be a multiple of 8 up to head_dim", rot);
   if (T == 0) return MONOFAB_OK;
-  if (!qkv || !positions || !slots || (rot && !cos_sin) || (hq && !q_out) || (hkv && (!k_cache || !v_cache)))
+  if (!a->qkv || !a->positions || !a->slots || (rot && !a->cos_sin) || (hq && !a->q_out) || (hkv && (!a->k_cache || !a->v_cache)))
     return fail(MONOFAB_EINVAL, "qk_rope: NULL argument");
-  if (max_pos < 1 || n_slots < 0) return fail(MONOFAB_EINVAL, "qk_rope: max_pos=%d, n_slots=%lld", max_pos, static_cast<long long>(n_slots));
-  if (!(eps >= 0.f)) return fail(MONOFAB_EINVAL, "qk_rope: eps must not be negative");
-  const uintptr_t at8 = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_cache) |
-                        reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(q_norm) | reinterpret_cast<uintptr_t>(k_norm);
-  if ((at8 & 7) || (reinterpret_cast<uintptr_t>(cos_sin) & 15) || (ld_qkv & 3) || (ld_out & 3))
+  if (a->max_pos < 1 || a->n_slots < 0) return fail(MONOFAB_EINVAL, "qk_rope: max_pos=%d, n_slots=%lld", a->max_pos, static_cast<long long>(a->n_slots));
+  if (!(a->eps >= 0.f)) return fail(MONOFAB_EINVAL, "qk_rope: eps must not be negative");
+  const uintptr_t at8 = reinterpret_cast<uintptr_t>(a->qkv) | reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->k_cache) |
+                        reinterpret_cast<uintptr_t>(a->v_cache) | reinterpret_cast<uintptr_t>(a->q_norm) | reinterpret_cast<uintptr_t>(a->k_norm);
+  if ((at8 & 7) || (reinterpret_cast<uintptr_t>(a->cos_sin) & 15) || ((a->ld_qkv | a->ld_out) & 3))
     return fail(MONOFAB_EINVAL, "qk_rope: rows must start at multiples of 8 bytes, the table at one of 16");
   QkRopeParams p{};
-  p.qkv = static_cast<const uint16_t*>(qkv);
-  p.positions = positions;
-  p.slots = slots;
-  p.cos_sin = cos_sin;
-  p.q_norm = static_cast<const uint16_t*>(q_norm);
-  p.k_norm = static_cast<const uint16_t*>(k_norm);
-  p.q_out = static_cast<uint16_t*>(q_out);
-  p.k_cache = static_cast<uint16_t*>(k_cache);
-  p.v_cache = static_cast<uint16_t*>(v_cache);
-  p.ld = ld_qkv;
-  p.ld_out = ld_out;
-  p.n_slots = n_slots;
+  p.qkv = static_cast<const uint16_t*>(a->qkv);
+  p.positions = a->positions;
+  p.slots = a->slots;
+  p.cos_sin = a->cos_sin;
+  p.q_norm = static_cast<const uint16_t*>(a->q_norm);
+  p.k_norm = static_cast<const uint16_t*>(a->k_norm);
+  p.q_out = static_cast<uint16_t*>(a->q_out);
+  p.k_cache = static_cast<uint16_t*>(a->k_cache);
+  p.v_cache = static_cast<uint16_t*>(a->v_cache);
+  p.ld = a->ld_qkv;
+  p.ld_out = a->ld_out;
+  p.n_slots = a->n_slots;
   p.T = T;
   p.hq = hq;
   p.hkv = hkv;
   p.rot = rot;
-  p.max_pos = max_pos;
-  p.interleaved = interleaved != 0;
-  p.eps = eps;
+  p.max_pos = a->max_pos;
+  p.interleaved = a->interleaved != 0;
+  p.eps = a->eps;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool wide = !(at8 & 15) && !((ld_qkv | ld_out) & 7);
+  const bool wide = !(at8 & 15) && !((a->ld_qkv | a->ld_out) & 7);
   auto go = [&](auto e) {
     using E = decltype(e);
-    return head_dim == 64 ? launch_qk_rope<E, 64>(p, wide, st) : head_dim == 128 ? launch_qk_rope<E, 128>(p, wide, st) : launch_qk_rope<E, 256>(p, wide, st);
+    return D == 64 ? launch_qk_rope<E, 64>(p, wide, st) : D == 128 ? launch_qk_rope<E, 128>(p, wide, st) : launch_qk_rope<E, 256>(p, wide, st);
   };
-  MF_CUDA(fp16 ? go(__half()) : go(__nv_bfloat16()));
+  MF_CUDA(a->fp16 ? go(__half()) : go(__nv_bfloat16()));
   return MONOFAB_OK;
 }
 

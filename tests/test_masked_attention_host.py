@@ -131,11 +131,24 @@ def test_cache_entry_points_refuse():
         assert rc == -1 and what in _C.lib.monofab_last_error(), (rc, _C.lib.monofab_last_error())
 
     lib = _C.lib
-    refused(b"head_dim", lib.monofab_qk_rope(at, 0, at, at, at, 1, None, None, at, 0, at, at, 1, 1, 1, 1, 96, 0, 0, 0, 1e-6, None))
-    refused(b"rot", lib.monofab_qk_rope(at, 0, at, at, at, 1, None, None, at, 0, at, at, 1, 1, 1, 1, 128, 12, 0, 0, 1e-6, None))
-    refused(b"NULL", lib.monofab_qk_rope(None, 0, at, at, at, 1, None, None, at, 0, at, at, 1, 1, 1, 1, 128, 128, 0, 0, 1e-6, None))
-    refused(b"8 bytes", lib.monofab_qk_rope(at + 2, 0, at, at, at, 1, None, None, at, 0, at, at, 1, 1, 1, 1, 128, 128, 0, 0, 1e-6, None))
-    refused(b"eps", lib.monofab_qk_rope(at, 0, at, at, at, 1, None, None, at, 0, at, at, 1, 1, 1, 1, 128, 128, 0, 0, float("nan"), None))
+    good = dict(qkv=at, positions=at, slots=at, cos_sin=at, q_out=at, k_cache=at, v_cache=at, n_slots=1, T=1, hq=1, hkv=1, head_dim=128, rot=128,
+                max_pos=1, eps=1e-6)
+
+    def rope(**kw):
+        return lib.monofab_qk_rope(ctypes.byref(_C.QkRopeArgsC(**{**good, **kw})), None)
+
+    refused(b"head_dim", rope(head_dim=96))
+    refused(b"rot", rope(rot=12))
+    refused(b"rot", rope(rot=136))
+    refused(b"NULL", rope(qkv=None))
+    refused(b"NULL", rope(v_cache=None))
+    refused(b"8 bytes", rope(qkv=at + 2))
+    refused(b"8 bytes", rope(ld_out=130))
+    refused(b"eps", rope(eps=float("nan")))
+    refused(b"max_pos", rope(max_pos=0))
+    refused(b"hq", rope(hq=1 << 17))
+    refused(b"NULL", lib.monofab_qk_rope(None, None))
+    assert rope(T=0) == 0
     refused(b"page_bytes", lib.monofab_page_copy(at, 1, at, at, 1, 1, 24, at, None))
     refused(b"65535", lib.monofab_page_copy(at, 1, at, at, 65536, 1, 32, at, None))
     refused(b"NULL", lib.monofab_page_copy(at, 1, at, None, 1, 1, 32, at, None))
@@ -144,6 +157,16 @@ def test_cache_entry_points_refuse():
     refused(b"NULL", lib.monofab_accept_rows(at, 1, at, 1, at, at, at, 1, 1, 16, 1, 16, None, None))
     assert lib.monofab_page_copy(at, 1, at, at, 0, 1, 32, at, None) == 0
     assert lib.monofab_accept_rows(at, 1, at, 1, at, at, at, 0, 1, 16, 1, 16, at, None) == 0
+
+
+def test_packed_arguments_are_the_structs():
+    """What the wrappers pack is laid out as the structs of the header."""
+    from monoserve_b200 import _C, attention, cache
+    for packer, struct in ((attention._masked_args, _C.MaskedAttentionArgsC), (cache._rope_args, _C.QkRopeArgsC)):
+        names = [n for n, _ in struct._fields_ if n != "reserved"]
+        a = struct.from_buffer_copy(packer.pack(*range(1, len(names) + 1)))
+        assert packer.size == ctypes.sizeof(struct)
+        assert [getattr(a, n) for n in names] == list(range(1, len(names) + 1))
 
 
 def test_cache_pages_refuse():

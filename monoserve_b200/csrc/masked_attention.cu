@@ -539,43 +539,43 @@ __device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
   uint32_t loads = 0;
   Records records;
   auto run = [&] {
-  while (const Record* const got = records.next(sh)) {
-    const Record rec = *got;   // in registers: the loops below would read it again behind every barrier
-    const int n = rec.t1 - rec.t0, lead = rec.pair ? 0 : 1;   // K runs one tile ahead of V where the streams take alternate tiles
-    const int32_t* const table = p.block_table + static_cast<size_t>(rec.req) * p.bt_stride;
-    int ahead = 0;   // this lane's page of the tile of `step`, and whether some row sees a key of it
-    bool there = false;
-    auto look_up = [&](int j) {
-      const int key = rec.tile_key(rec.t0 + j) + lane * p.page;
-      there = lane < pages && key < rec.hi && (key + p.page > rec.lo || key < rec.near);
-      ahead = there ? table[key / p.page] : 0;
-    };
-    int last_page = 0;
-    bool last_there = false;
-    auto load = [&](const CUtensorMap* map, int page, bool wanted) {
-      if (!wait_for(&sh.kv_empty[ring.stage], ring.phase ^ 1, &sh.abort_flag)) return false;
-      const uint32_t which = __ballot_sync(0xffffffffu, wanted);
-      if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[ring.stage], __popc(which) * page_bytes);
-      __syncwarp();
-      if (wanted) load_box_5d(ring_mem + ring.stage * L::kTileBytes + lane * page_bytes, map, &sh.kv_full[ring.stage], L::kHalves * rec.head, page);
-      ring.advance();
-      ++loads;
-      return true;
-    };
-    for (int step = 0; step < n + lead; ++step) {
-      if (step < n) {
-        look_up(step);
-        if (!load(&p.k_map, ahead, there)) return;
-      }
-      if (lead == 0) {
-        if (!load(&p.v_map, ahead, there)) return;
-      } else {
-        if (step > 0 && !load(&p.v_map, last_page, last_there)) return;
-        last_page = ahead;
-        last_there = there;
+    while (const Record* const got = records.next(sh)) {
+      const Record rec = *got;   // in registers: the loops below would read it again behind every barrier
+      const int n = rec.t1 - rec.t0, lead = rec.pair ? 0 : 1;   // K runs one tile ahead of V where the streams take alternate tiles
+      const int32_t* const table = p.block_table + static_cast<size_t>(rec.req) * p.bt_stride;
+      int ahead = 0;   // this lane's page of the tile of `step`, and whether some row sees a key of it
+      bool there = false;
+      auto look_up = [&](int j) {
+        const int key = rec.tile_key(rec.t0 + j) + lane * p.page;
+        there = lane < pages && key < rec.hi && (key + p.page > rec.lo || key < rec.near);
+        ahead = there ? table[key / p.page] : 0;
+      };
+      int last_page = 0;
+      bool last_there = false;
+      auto load = [&](const CUtensorMap* map, int page, bool wanted) {
+        if (!wait_for(&sh.kv_empty[ring.stage], ring.phase ^ 1, &sh.abort_flag)) return false;
+        const uint32_t which = __ballot_sync(0xffffffffu, wanted);
+        if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[ring.stage], __popc(which) * page_bytes);
+        __syncwarp();
+        if (wanted) load_box_5d(ring_mem + ring.stage * L::kTileBytes + lane * page_bytes, map, &sh.kv_full[ring.stage], L::kHalves * rec.head, page);
+        ring.advance();
+        ++loads;
+        return true;
+      };
+      for (int step = 0; step < n + lead; ++step) {
+        if (step < n) {
+          look_up(step);
+          if (!load(&p.k_map, ahead, there)) return;
+        }
+        if (lead == 0) {
+          if (!load(&p.v_map, ahead, there)) return;
+        } else {
+          if (step > 0 && !load(&p.v_map, last_page, last_there)) return;
+          last_page = ahead;
+          last_there = there;
+        }
       }
     }
-  }
   };
   run();
   // however it ended, the last loads have landed before the CTA's memory is given up
@@ -595,7 +595,7 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
   constexpr uint32_t idesc_s = idesc_of<E>(kTile), idesc_o = idesc_of<E>(D) | (1u << 16);   // V is MN-major
   Ring<L::kStages> ring;
   Records records;
-  uint32_t q_count = 0, p_count[2] = {0, 0};
+  uint32_t q_count = 0, p_phase = 0;   // p_phase: bit x, the parity of stream x's next weights
   auto wait_stage = [&] { return wait_for(&sh.kv_full[ring.stage], ring.phase, &sh.abort_flag); };
   auto release = [&](int stage) {
     if (leader) umma_commit(&sh.kv_empty[stage]);
@@ -611,14 +611,14 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
   };
   auto values = [&](int x, int stage, bool accumulate) {   // O[x] (+)= P[x] V
     const uint32_t v = (smem_u32(ring_mem) + stage * L::kTileBytes) >> 4 | 64u << 16;
-    if (!wait_for(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag)) return false;
+    if (!wait_for(&sh.p_full[x], p_phase >> x & 1, &sh.abort_flag)) return false;
+    p_phase ^= 1u << x;
     tc_fence_after_sync();
     if (leader) {
 #pragma unroll
       for (int i = 0; i < kTile / 16; ++i)
         umma_tmem_a(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, smem_desc(v + i * (L::kGroupBytes / 8), L::kGroupBytes), idesc_o, accumulate || i != 0);
     }
-    ++p_count[x];
     return true;
   };
   // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none.
@@ -657,8 +657,8 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
       const int x = j & 1;
       if (!wait_stage()) return false;
       clean(rec, ring.stage, rec.t0 + j);
-      if (!wait_for(&sh.p_full[x], p_count[x] & 1, &sh.abort_flag)) return false;
-      ++p_count[x];
+      if (!wait_for(&sh.p_full[x], p_phase >> x & 1, &sh.abort_flag)) return false;
+      p_phase ^= 1u << x;
       tc_fence_after_sync();
       if (leader) {
         const uint32_t v = (smem_u32(ring_mem) + ring.stage * L::kTileBytes) >> 4 | 64u << 16;

@@ -20,11 +20,12 @@
 //   * The work is shared out on the device, from lengths that are read there: tiles and items have a cost (below), every
 //     CTA takes an equal part of its sum, and items that a border cuts leave 32-bit rows and (reference, sum) in a workspace,
 //     which a second kernel joins in order: the same bits every time. A border near an item's begin is moved there.
-//   * A tile that all rows of a stream see goes without masks; else a row has the tile's keys as bits: the ranges of the window
-//     and the sinks, or the past and the tree's bits, shifted. Pages that no row of the item sees are not loaded, and values that
+//   * An item's tiles are cut from the pages that its rows see, one behind the other: those of the sinks, then those of the window. A
+//     tile that all rows of a stream see goes without masks; else a row has the tile's keys as bits: the ranges of the window and the
+//     sinks, or the past and the tree's bits, shifted. Pages that no row of the item sees are not loaded, and values that
 //     none sees are zeroed in shared memory, so that nothing there can reach a sum.
 //
-// What bounds it (B200, clocks as they come): contexts of single tokens HBM, 5.6 TB/s of K and V (128 sequences, 843 MB: 151 us);
+// What bounds it (B200, clocks as they come): contexts of single tokens HBM, 5.7 TB/s of K and V (128 sequences, 843 MB: 147 us);
 // prompts and large trees the softmax: a pair's tile takes 3400 cycles, of which its products take 2048 and the exponentials of both
 // streams 2048 of the special-function units, one stream's rows 2050 from S to P and 1350 from P to the next S. Measured and dropped: a row
 // of S in registers (straight-line code for 128 columns is bound by its fetch: long trees 448 -> 505 us), sixteen warps of softmax
@@ -107,11 +108,13 @@ __device__ __forceinline__ Request request_of(const Params& p, int r) {
 }
 __device__ __forceinline__ int blocks_of(const Params& p, int rows) { return (rows + 2 * p.per_stream - 1) / (2 * p.per_stream); }
 
-// The keys that the rows of a block see lie in [0, near) and [lo, hi); they are covered by sink_tiles tiles from 0 on and by
-// win_tiles from tile win_tile0 on.
+// The keys that the rows of a block see lie in [0, near) and [lo, hi). An item's tiles are 128 places in a row: first the pages of the
+// former, `split` places, then those of the latter; place v is key v below `split` and key v + shift from there on. (Where the two meet
+// in a page, and for trees, places are keys.) lo, hi and near are places.
+// (Tiles at multiples of 128 keys, the sinks in one of their own: window prompts with 4 sinks 157 us, so 141.)
 struct Span {
-  int tokens, pos0, lo, hi, near, sink_tiles, win_tile0, win_tiles;
-  __device__ __forceinline__ int tiles() const { return sink_tiles + win_tiles; }
+  int tokens, pos0, lo, hi, near, split, shift;
+  __device__ __forceinline__ int tiles() const { return (hi + kTile - 1) / kTile; }
   __device__ __forceinline__ int tile_cost(const Params& p) const { return tokens > p.per_stream ? kPairCost : 1; }
   __device__ __forceinline__ int cost(const Params& p) const { return tiles() * tile_cost(p) + kItemCost; }
 };
@@ -121,17 +124,19 @@ __device__ __forceinline__ Span span_of(const Params& p, const Request& q, int b
   s.tokens = min(2 * p.per_stream, q.rows - first);
   s.pos0 = q.kv_len - q.rows + first;
   const int there = min(q.kv_len, p.bt_stride * p.page);
-  if (p.tree) {
-    s.lo = s.near = 0;
-    s.hi = there;
-  } else {
-    s.hi = max(0, min(there, s.pos0 + s.tokens));
-    s.lo = static_cast<int>(max(0ll, static_cast<long long>(s.pos0) - p.window + 1));
-    s.near = min(min(p.sinks, s.hi), s.lo);
+  s.near = s.lo = s.split = s.shift = 0;
+  s.hi = there;
+  if (p.tree) return s;
+  s.hi = max(0, min(there, s.pos0 + s.tokens));
+  const int lo = static_cast<int>(max(0ll, static_cast<long long>(s.pos0) - p.window + 1));
+  s.near = min(min(p.sinks, s.hi), lo);
+  const int split = (s.near + p.page - 1) / p.page * p.page, from = lo / p.page * p.page;
+  if (split < from) {
+    s.split = split;
+    s.shift = from - split;
   }
-  s.win_tile0 = s.lo / kTile;
-  s.win_tiles = max(0, (s.hi + kTile - 1) / kTile - s.win_tile0);
-  s.sink_tiles = min((s.near + kTile - 1) / kTile, s.win_tile0);
+  s.lo = lo - s.shift;
+  s.hi = max(s.near, s.hi - s.shift);   // below lo where the window has no key that is there
   return s;
 }
 
@@ -144,12 +149,11 @@ __device__ __forceinline__ bool same_item(const Place& a, const Place& b) { retu
 // One part of an item, as the roles get it.
 struct Record {
   int req, head, row0, tokens, pos0, past, there;   // there: keys in the block table; past: first drafted key
-  int lo, hi, near;
-  int sink_tiles, win_tile0, t0, t1;
+  int lo, hi, near, split, shift;                   // of its Span
+  int t0, t1;
   int slot;     // -1: the whole item, else the workspace slot
   int pair;     // two streams of rows; else the streams take alternate tiles. -1: no more items
   int few;      // not a pair, and few enough rows to be the columns of the scores (kFewRows)
-  __device__ __forceinline__ int tile_key(int t) const { return kTile * (t < sink_tiles ? t : t - sink_tiles + win_tile0); }
 };
 
 template <int D>
@@ -456,8 +460,8 @@ __device__ void schedule(const Params& p, Shared& sh, uint8_t* q_mem) {
       rec.lo = s.lo;
       rec.hi = s.hi;
       rec.near = s.near;
-      rec.sink_tiles = s.sink_tiles;
-      rec.win_tile0 = s.win_tile0;
+      rec.split = s.split;
+      rec.shift = s.shift;
       rec.t0 = at.t;
       rec.t1 = same_item(at, end) ? end.t : tiles;
       const int cta = static_cast<int>(blockIdx.x);
@@ -525,8 +529,8 @@ struct Ring {
   }
 };
 
-// Whether any row of the item sees key `key`.
-__device__ __forceinline__ bool some_row_sees(const Record& rec, int key) { return key < rec.hi && (key >= rec.lo || key < rec.near); }
+// Whether any row of the item sees the key at a place.
+__device__ __forceinline__ bool some_row_sees(const Record& rec, int place) { return place < rec.near || (place >= rec.lo && place < rec.hi); }
 
 // ------------------------------------------------------------------------------------------------------ the roles
 
@@ -546,9 +550,9 @@ __device__ void produce(const Params& p, Shared& sh, uint8_t* ring_mem) {
       int ahead = 0;   // this lane's page of the tile of `step`, and whether some row sees a key of it
       bool there = false;
       auto look_up = [&](int j) {
-        const int key = rec.tile_key(rec.t0 + j) + lane * p.page;
-        there = lane < pages && key < rec.hi && (key + p.page > rec.lo || key < rec.near);
-        ahead = there ? table[key / p.page] : 0;
+        const int place = (rec.t0 + j) * kTile + lane * p.page;
+        there = lane < pages && (place < rec.near || (place + p.page > rec.lo && place < rec.hi));
+        ahead = there ? table[(place < rec.split ? place : place + rec.shift) / p.page] : 0;
       };
       int last_page = 0;
       bool last_there = false;
@@ -623,12 +627,12 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
   };
   // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none.
   auto clean = [&](const Record& rec, int stage, int t) {
-    const int key0 = rec.tile_key(t);
-    if (key0 + kTile <= rec.hi && (key0 >= rec.lo || key0 + kTile <= rec.near)) return;
+    const int place0 = t * kTile;
+    if (place0 + kTile <= rec.near || (place0 >= rec.lo && place0 + kTile <= rec.hi)) return;
     uint8_t* const v = ring_mem + stage * L::kTileBytes;
     for (int i = lane / 8; i < kTile * L::kHalves; i += 4) {
       const int k = i / L::kHalves;
-      if (!some_row_sees(rec, key0 + k))
+      if (!some_row_sees(rec, place0 + k))
         *reinterpret_cast<uint4*>(v + (k >> 3) * L::kGroupBytes + (i % L::kHalves) * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
     }
     fence_proxy_async_smem();
@@ -802,7 +806,7 @@ __device__ bool softmax_few(const Params& p, Shared& sh, uint8_t* q_mem, const R
     if (!wait_for(&sh.s_full[wg], c.s & 1, &sh.abort_flag)) return false;
     ++c.s;
     tc_fence_after_sync();
-    const int key0 = rec.tile_key(rec.t0 + j), key = key0 + r;
+    const int place0 = (rec.t0 + j) * kTile, place = place0 + r, key = place < rec.split ? place : place + rec.shift;
     float s[N];
     {
       uint32_t v[N];
@@ -812,9 +816,9 @@ __device__ bool softmax_few(const Params& p, Shared& sh, uint8_t* q_mem, const R
       for (int i = 0; i < N; ++i) s[i] = __uint_as_float(v[i]) * scale;
     }
     bool full;
-    if (p.tree) full = key0 + kTile <= min(rec.past, rec.there);
-    else full = key0 + kTile <= min(rec.pos0 + 1, rec.there) &&
-                (key0 >= static_cast<long long>(rec.pos0) + rec.tokens - p.window || key0 + kTile <= p.sinks);
+    if (p.tree) full = place0 + kTile <= min(rec.past, rec.there);
+    else full = place0 + kTile <= rec.near || (place0 + kTile + rec.shift <= min(rec.pos0 + 1, rec.there) &&
+                                               static_cast<long long>(place0) + rec.shift >= static_cast<long long>(rec.pos0) + rec.tokens - p.window);
     if (!full) {
       uint32_t seen = 0;   // the rows that see the key
       const uint32_t token = (1u << p.group) - 1u;
@@ -965,12 +969,11 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
     const int tokens = min(rec.tokens - first, p.per_stream);
     const bool row_ok = r < tokens * p.group;
     const bool works = quad * 32 < tokens * p.group;                           // warp-uniform
-    // first keys of the tiles that all rows of the stream see: up to full_hi, from full_lo on or up to full_near
+    // first places of the tiles that all rows of the stream see: from full_lo to full_hi, or up to full_near
     const int pos_first = rec.pos0 + first;
-    const int full_hi = min(p.tree ? rec.past : pos_first + 1, rec.there) - kTile;
-    const int full_lo = p.tree ? 0 : static_cast<int>(max(0ll, static_cast<long long>(pos_first + tokens) - p.window));
-    const int full_near = p.tree ? 0 : p.sinks - kTile;
-    const int key_base = rec.t0 * kTile, sinks_end = rec.sink_tiles * kTile, jump = (rec.win_tile0 - rec.sink_tiles) * kTile;
+    const int full_hi = min(p.tree ? rec.past : pos_first + 1, rec.there) - rec.shift - kTile;
+    const int full_lo = p.tree ? 0 : static_cast<int>(max(0ll, static_cast<long long>(pos_first + tokens) - p.window)) - rec.shift;
+    const int full_near = rec.near - kTile;
     float m = -INFINITY, l = 0.f;
     bool begun = false;
 #pragma unroll 1
@@ -983,25 +986,27 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
         mbar_arrive(&sh.p_full[wg]);
         continue;
       }
-      int key0 = key_base + j * kTile;
-      if (key0 >= sinks_end) key0 += jump;
-      const bool full = key0 <= full_hi && (key0 >= full_lo || key0 <= full_near);
+      const int place0 = (rec.t0 + j) * kTile;
+      const bool full = place0 <= full_near || (place0 <= full_hi && place0 >= full_lo);
       uint32_t seen[4];   // what the row sees of the tile
       if (!full) {
         if (p.tree) {
           const int32_t* const words = p.tree + static_cast<size_t>(rec.row0 + (row_ok ? first + token_in : 0)) * p.words;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int d = key0 + 32 * c - rec.past;   // the drafted token of the first column
+            const int d = place0 + 32 * c - rec.past;   // the drafted token of the first column; places are keys
             const int w = d >> 5, s = d & 31;         // floor
             const uint32_t a = w >= 0 && w < p.words ? words[w] : 0u, b = w + 1 >= 0 && w + 1 < p.words ? words[w + 1] : 0u;
-            seen[c] = (__funnelshift_r(a, b, s) | bits_of(0, -d)) & bits_of(0, rec.there - key0 - 32 * c);
+            seen[c] = (__funnelshift_r(a, b, s) | bits_of(0, -d)) & bits_of(0, rec.there - place0 - 32 * c);
           }
         } else {
           const int pos = pos_first + token_in;
-          const int hi = max(0, min(min(pos + 1, rec.there) - key0, kTile));
-          const int lo = static_cast<int>(max(0ll, min(static_cast<long long>(pos) - p.window + 1 - key0, static_cast<long long>(kTile))));
-          const int near = static_cast<int>(min(max(0ll, static_cast<long long>(p.sinks) - key0), static_cast<long long>(hi)));
+          // as places: the window's keys lie behind the split, where place = key - shift; what is near lies in front of it, or
+          // there is no split and the row's own sinks may reach into the window of an earlier one
+          const long long origin = static_cast<long long>(place0) + rec.shift;
+          const int hi = static_cast<int>(max(0ll, min(min(static_cast<long long>(pos) + 1, static_cast<long long>(rec.there)) - origin, static_cast<long long>(kTile))));
+          const int lo = static_cast<int>(max(0ll, min(static_cast<long long>(pos) - p.window + 1 - origin, static_cast<long long>(kTile))));
+          const int near = rec.split ? rec.near - place0 : min(p.sinks - place0, rec.shift ? 0 : hi);
 #pragma unroll
           for (int c = 0; c < 4; ++c) seen[c] = bits_of(lo - 32 * c, hi - 32 * c) | bits_of(0, near - 32 * c);
         }

@@ -16,7 +16,7 @@
 //   * Warps: 0 loads K and V through a ring of 32 or 16 KB stages; 1 issues the products; 2 hands out items and loads queries; 4 - 7
 //     and 8 - 11 are the streams' softmax, a thread a row. One warp issues both streams' products: it keeps them a step apart, so
 //     that one's products run under the other's softmax. (A warp for each: their products run into each other, both streams wait at the
-//     same time; window prompts 177 -> 187 us.)
+//     same time.)
 //   * The work is shared out on the device, from lengths that are read there: tiles and items have a cost (below), every
 //     CTA takes an equal part of its sum, and items that a border cuts leave 32-bit rows and (reference, sum) in a workspace,
 //     which a second kernel joins in order: the same bits every time. A border near an item's begin is moved there.
@@ -26,11 +26,13 @@
 //     none sees are zeroed in shared memory, so that nothing there can reach a sum.
 //
 // What bounds it (B200, clocks as they come): contexts of single tokens HBM, 5.7 TB/s of K and V (128 sequences, 843 MB: 147 us);
-// prompts and large trees the softmax: a pair's tile takes 3400 cycles, of which its products take 2048 and the exponentials of both
-// streams 2048 of the special-function units, one stream's rows 2050 from S to P and 1350 from P to the next S. Measured and dropped: a row
-// of S in registers (straight-line code for 128 columns is bound by its fetch: long trees 448 -> 505 us), sixteen warps of softmax
-// (500 -> 530), half tiles with two score buffers a stream (467; its scores cost half as much again), weights handed over in two parts (no
-// change), the next columns' TMEM loads ahead of the weights (469 -> 500).
+// prompts and large trees the chain of a stream's tile and the card's power: 3350 cycles, 1900 from S to P (maxima 280, weights 1400) and 1450
+// from P to the next S (values 512, scores 512, hand-overs); window prompts 129 us, long trees 420 in short runs and 530 in long ones.
+// The loop of tiles is short on purpose: a warp's instructions come from a small cache, and every one that the loop does not need shows
+// (masks in the loops of maxima and weights instead of ahead of them: 141 us). Measured and dropped: a row of S in registers (234), two chunks of
+// weights in line (134), the next columns' TMEM loads ahead of the weights (177 -> 201 at the time), sixteen warps of softmax (177 -> 206),
+// half tiles with two score buffers a stream (177 -> 191; the scores cost half as much again), a warp for each stream's products (177 -> 187),
+// weights handed over in two parts (128).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -64,7 +66,7 @@ constexpr int kMaxRequests = 16384;
 constexpr int kFewRows = 16, kFewBytes = 2 * kFewRows * 128;   // kFewBytes: weights of such a stream, two times 64 keys of a row in 128 bytes
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr float kSlack = 8.f;
-constexpr int kByFma = 4;           // weights of 32 worked out by multiplications
+constexpr int kByFma = 8;           // weights of 32 worked out by multiplications
 
 // Where a call that names no status word leaves its bits.
 __device__ int g_masked_attention_status;
@@ -111,7 +113,7 @@ __device__ __forceinline__ int blocks_of(const Params& p, int rows) { return (ro
 // The keys that the rows of a block see lie in [0, near) and [lo, hi). An item's tiles are 128 places in a row: first the pages of the
 // former, `split` places, then those of the latter; place v is key v below `split` and key v + shift from there on. (Where the two meet
 // in a page, and for trees, places are keys.) lo, hi and near are places.
-// (Tiles at multiples of 128 keys, the sinks in one of their own: window prompts with 4 sinks 157 us, so 141.)
+// (Tiles at multiples of 128 keys, the sinks in one of their own: window prompts with 4 sinks 157 us where this took 141.)
 struct Span {
   int tokens, pos0, lo, hi, near, split, shift;
   __device__ __forceinline__ int tiles() const { return (hi + kTile - 1) / kTile; }
@@ -318,8 +320,7 @@ __device__ __forceinline__ float2 exp2_by_fma(Pair x) {
 }
 
 // The weights of 32 scores, packed, and added to `sum`. kByFma of them are worked out by multiplications: the special-function unit
-// gives 16 a cycle and SM, as long for a tile as its matrix products. (None: long trees 466 us, window prompts 169; 4: 457, 166;
-// 8: 458, 167, and decode batches 1 % longer.)
+// gives 16 a cycle and SM, as long for a tile as its matrix products. (None: window prompts 136 us; 4: 130.5; 8: 129; 12: 129.)
 template <class E>
 __device__ __forceinline__ void weigh(const uint32_t (&v)[32], float scale, float shift, Pair& sum, uint32_t (&out)[16]) {
   const Pair scales = pair_of(scale, scale), shifts = pair_of(shift, shift);
@@ -343,14 +344,6 @@ __device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
   lo = max(lo, 0), hi = min(hi, 32);
   if (lo >= hi) return 0u;
   return (0xffffffffu >> (32 - (hi - lo))) << lo;
-}
-
-// Of 32 scores, those whose bit is not set become as low as can be. The border of a window or of the past lies in one or two of a
-// tile's four chunks.
-__device__ __forceinline__ void hide(uint32_t* v, uint32_t seen) {
-  if (__all_sync(0xffffffffu, seen == 0xffffffffu)) return;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = seen >> i & 1u ? v[i] : 0xff800000u;
 }
 
 // ---------------------------------------------------------------------------------------------------- the shares
@@ -1011,18 +1004,28 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
           for (int c = 0; c < 4; ++c) seen[c] = bits_of(lo - 32 * c, hi - 32 * c) | bits_of(0, near - 32 * c);
         }
       }
-      // The parts of a row one after the other through the same code: straight-line code for all 128 columns is bound by its fetch.
-      float mx = -INFINITY;
+      if (!full) {   // what the row does not see is hidden in TMEM, so that the loops below need not know
 #pragma unroll 1
+        for (int c = 0; c < kTile; c += 32) {
+          const uint32_t bits = c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3]);
+          if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;   // a border lies in one or two of the four chunks
+          uint32_t v[32];
+          tmem_ld_32x32(tmem_s + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = bits >> i & 1u ? v[i] : 0xff800000u;
+          store_tmem_16(tmem_s + c, v);
+          store_tmem_16(tmem_s + c + 16, v + 16);
+        }
+        store_tmem_wait();
+      }
+      float mx = -INFINITY;
+#pragma unroll
       for (int c = 0; c < kTile; c += 64) {
         uint32_t v[64];
         tmem_ld_32x32(tmem_s + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
         tmem_ld_32x32(tmem_s + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
         tmem_ld_wait();
-        if (!full) {
-          hide(&v[0], c ? seen[2] : seen[0]);
-          hide(&v[32], c ? seen[3] : seen[1]);
-        }
         float top[4] = {mx, mx, mx, mx};
 #pragma unroll
         for (int i = 0; i < 64; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
@@ -1058,7 +1061,6 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
         uint32_t v[32], w[16];
         tmem_ld_32x32(tmem_s + c, v);
         tmem_ld_wait();
-        if (!full) hide(v, c < 64 ? (c < 32 ? seen[0] : seen[1]) : (c < 96 ? seen[2] : seen[3]));
         weigh<E>(v, scale, shift, sum, w);
         store_tmem_16(tmem_s + c / 2, w);
       }
@@ -1442,7 +1444,7 @@ extern "C" int monofab_masked_attention(const monofab_masked_attention_args* a, 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Batches of single tokens and the like (by the mean of their rows: what the host knows) take the kernel that also has a form for items
   // of few rows. 128 single tokens over 843 MB, long runs: 153 us, without the form 177 (at the card's power limit: 128 rows of products
-  // for eight that are there); but its code alone, unused, makes window prompts 157 -> 162.
+  // for eight that are there); but its code alone, unused, made window prompts 157 -> 162.
   const bool few = static_cast<int64_t>(a->tokens) * group <= static_cast<int64_t>(a->requests) * kFewRows;
   auto go = [&](auto e) {
     using E = decltype(e);

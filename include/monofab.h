@@ -140,8 +140,8 @@ int monofab_attention(const void* q, const void* k_cache, const void* v_cache, v
  *   else           the past (j < kv_len - rows) and the drafted tokens whose bit is set: of drafted token d bit d % 32 of
  *                  tree[row][d / 32]; those from 32 * words on have none.
  * out = sum_j softmax_j(scale q k_j) v_j; a row that sees no key is zeros.  Rows of no request keep what they hold.
- * Keys and values of drafted tokens, and of what any row of a request sees, must be finite, also for that request's rows that
- * do not see them; what no row of a request sees may hold anything.  At most 16384 requests a call.
+ * Values that some row of a request sees must be finite, also for that request's rows that do not see them; what no row sees
+ * may hold anything.  A row that sees a score that is infinite or no number is NaN.  At most 16384 requests a call.
  * Keys past the block table (kv_len > bt_stride * page_size) are not there; a page number outside [0, n_pages) reads as
  * zeros; q_start is taken as ascending within [0, tokens], and a request that it gives no rows has none. */
 typedef struct {
@@ -194,7 +194,7 @@ int monofab_qk_rope(const monofab_qk_rope_args* args, void* stream);
 /* Page dst[i] takes what page src[i] holds, in all n_tensors cache tensors (device array of addresses, each
  * [n_pages][page_bytes], 16-byte aligned).  A pair whose page numbers lie outside [0, n_pages), whose destination is
  * another pair's source or destination or whose source is another's destination is not copied, and `status` (device
- * int32) receives MONOFAB_STATUS_BAD_ARGS.  At most 65535 pairs and tensors. */
+ * int32) receives MONOFAB_STATUS_BAD_ARGS.  A page and itself are a pair that does nothing (padding).  At most 65535 pairs and tensors. */
 int monofab_page_copy(const uint64_t* tensors, int n_tensors, const int32_t* src, const int32_t* dst, int pairs, int n_pages,
                       int64_t page_bytes, int32_t* status, void* stream);
 

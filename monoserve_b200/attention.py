@@ -160,6 +160,11 @@ def _refuse(ok, what):
     ok or _no(what)
 
 
+def _stream_of(index, stream):
+    stream is None or stream.device.index == index or _no("the stream belongs to another device than the tensors")
+    return stream
+
+
 @functools.lru_cache(maxsize=None)
 def _masked_ws_bytes(device_index, head_dim):
     n = _C.lib.monofab_masked_attention_ws_bytes(head_dim)
@@ -213,7 +218,7 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
         (out is None or out.get_device() == index) and (status is None or status.get_device() == index) or _no("all tensors must be on one CUDA device")
     status is None or (status.dtype == torch.int32 and status.numel() >= 1) or _no("status is int32")
     if stream is not None or torch.cuda.current_device() != index:
-        with torch.cuda.device(index), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
+        with torch.cuda.device(index), torch.cuda.stream(_stream_of(index, stream)):   # what is allocated in the call belongs to its stream
             return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window, sinks, tree, scale, out, None, status)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
@@ -239,8 +244,9 @@ def sliding_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     q_start[r] .. q_start[r + 1] - 1; kv_len int32 [requests]: its keys, those of its rows the last of them.  The lengths are read
     on the device: a call captured in a CUDA graph can be replayed with others.  Returns [T, hq, D] (`out`, which may be q
     itself): rows that see no key are zeros, rows of no request keep what they hold (are undefined in a new tensor).
-    A bounded wait that ran out is reported in `status` (int32 on the device), or to attention_status().  Keys that some row of
-    a request sees must hold finite values; the others may hold anything.  At most 16384 requests."""
+    A bounded wait that ran out is reported in `status` (int32 on the device), or to attention_status().  Values that some row
+    of a request sees must be finite; what none sees may hold anything.  A score that is infinite or no number makes the rows
+    that see it NaN.  At most 16384 requests."""
     return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, int(window), int(sinks), None, scale, out, stream, status)
 
 

@@ -27,7 +27,7 @@
 //
 // What bounds it (B200, clocks as they come): contexts of single tokens HBM, 5.7 TB/s of K and V (128 sequences, 843 MB: 147 us);
 // prompts and large trees the chain of a stream's tile and the card's power: 3350 cycles, 1900 from S to P (maxima 280, weights 1400) and 1450
-// from P to the next S (values 512, scores 512, hand-overs); window prompts 129 us, long trees 420 in short runs and 530 in long ones.
+// from P to the next S (values 512, scores 512, hand-overs); window prompts 131 us, long trees 425 in short runs and 530 in long ones.
 // The loop of tiles is short on purpose: a warp's instructions come from a small cache, and every one that the loop does not need shows
 // (masks in the loops of maxima and weights instead of ahead of them: 141 us). Measured and dropped: a row of S in registers (234), two chunks of
 // weights in line (134), the next columns' TMEM loads ahead of the weights (177 -> 201 at the time), sixteen warps of softmax (177 -> 206),
@@ -42,8 +42,8 @@
 #include <cmath>
 #include <type_traits>
 
+#include "../../include/monofab.h"
 #include "kernels.h"
-#include "masked_attention.h"
 #include "moe_layer.h"
 #include "ptx.cuh"
 
@@ -235,9 +235,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 // Two 32-bit values as one operand of the packed instructions.
@@ -522,8 +522,37 @@ struct Ring {
   }
 };
 
-// Whether any row of the item sees the key at a place.
-__device__ __forceinline__ bool some_row_sees(const Record& rec, int place) { return place < rec.near || (place >= rec.lo && place < rec.hi); }
+// Values in a tile of keys that no row of the item sees become zeros, by a warp: their weights are, but zero times infinity is none.
+// tree: of the item's first token, or NULL. Runs while the tile's weights are worked out, and apart from the loop of tiles, which pays for
+// every instruction (window prompts 131 us; in line 133, as two functions around the wait for the values 136).
+template <int D>
+__device__ __noinline__ void clean_values(const int32_t* tree, int words, int tokens, int past, int near, int lo, int hi, int place0, uint8_t* v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    const int at = place0 + c, d = at - past;   // d: the drafted token of the first key
+    uint32_t seen = bits_of(lo - at, hi - at) | bits_of(0, near - at);
+    if (tree && d + 32 > 0) {
+      const int w = d >> 5, s = d & 31;   // floor; w >= -1
+      uint32_t some = 0;
+      for (int t = lane; t < tokens; t += 32) {
+        const int32_t* const row = tree + static_cast<size_t>(t) * words;
+        const uint32_t a = w >= 0 && w < words ? row[w] : 0u, b = w + 1 < words ? row[w + 1] : 0u;
+        some |= __funnelshift_r(a, b, s);
+      }
+      seen &= __reduce_or_sync(0xffffffffu, some) | bits_of(0, -d);
+    }
+    if (seen == 0xffffffffu) continue;
+    for (int k = lane / 8; k < 32; k += 4) {
+      if (seen >> k & 1u) continue;
+#pragma unroll
+      for (int h = 0; h < Layout<D>::kHalves; ++h)
+        *reinterpret_cast<uint4*>(v + ((c + k) >> 3) * Layout<D>::kGroupBytes + h * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
 
 // ------------------------------------------------------------------------------------------------------ the roles
 
@@ -618,18 +647,11 @@ __device__ void multiply(const Params& p, Shared& sh, uint8_t* q_mem, uint8_t* r
     }
     return true;
   };
-  // Values of keys that no row sees become zeros: their weights are, but zero times infinity is none.
   auto clean = [&](const Record& rec, int stage, int t) {
-    const int place0 = t * kTile;
-    if (place0 + kTile <= rec.near || (place0 >= rec.lo && place0 + kTile <= rec.hi)) return;
-    uint8_t* const v = ring_mem + stage * L::kTileBytes;
-    for (int i = lane / 8; i < kTile * L::kHalves; i += 4) {
-      const int k = i / L::kHalves;
-      if (!some_row_sees(rec, place0 + k))
-        *reinterpret_cast<uint4*>(v + (k >> 3) * L::kGroupBytes + (i % L::kHalves) * 1024 + (k & 7) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
+    const int place0 = t * kTile, alike = p.tree ? min(rec.hi, rec.past) : rec.hi;
+    if (place0 + kTile <= rec.near || (place0 >= rec.lo && place0 + kTile <= alike)) return;
+    clean_values<D>(p.tree ? p.tree + static_cast<size_t>(rec.row0) * p.words : nullptr, p.words, rec.tokens, rec.past, rec.near, rec.lo, rec.hi, place0,
+                    ring_mem + stage * L::kTileBytes);
   };
   // An item of few rows: S^T[x] = K Q^T and O^T[x] (+)= V^T P^T[x]. Apart from the others, whose loop pays for every instruction.
   auto run_few = [&](const Record& rec, int n) {
@@ -904,7 +926,7 @@ __device__ bool softmax_few(const Params& p, Shared& sh, uint8_t* q_mem, const R
     sums[1] += sh.few.sum[1][q][at];
   }
   const float total = sums[0] * ea + sums[1] * eb;
-  const float inv = rec.slot >= 0 ? 1.f : total > 0.f ? 1.f / total : 0.f;
+  const float inv = rec.slot >= 0 ? 1.f : total == 0.f ? 0.f : 1.f / total;
   // where row `lane` goes; the streams' threads store every other row
   const int token = at / p.group, head = rec.head * p.group + at - token * p.group;
   unsigned long long to = 0;
@@ -1028,10 +1050,11 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
         tmem_ld_wait();
         float top[4] = {mx, mx, mx, mx};
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-        mx = max3(fmaxf(top[0], top[1]), top[2], top[3]);
+        for (int i = 0; i < 64; i += 2) top[i / 2 & 3] = max3_or_nan(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        mx = max3_or_nan(max_or_nan(top[0], top[1]), top[2], top[3]);
       }
       mx *= scale;
+      if (!(mx < INFINITY)) l = NAN;   // not left to the weights: those by multiplications make a number of it
       // The point that a row's exponentials refer to moves when its maximum has grown past it by more than kSlack: weights stay
       // below 2^kSlack, and O is rarely rescaled. S of this tile is there, so P V of the stream's tile before it is, too.
       if (!begun) {
@@ -1096,7 +1119,7 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
       c1 = c0 + D / 2;
       other = 128;
     }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
     const uint32_t from = tmem_o + (rec.pair ? wg * 128 : 0);
     if (works) {
 #pragma unroll 1
@@ -1316,7 +1339,7 @@ __global__ void __launch_bounds__(256) masked_join_kernel(const __grid_constant_
     for (int j = 0; j < kRows; ++j) {
       const int i = i0 + j * warps;
       if (i >= n) break;
-      const float inv = sum[j] > 0.f ? 1.f / sum[j] : 0.f;
+      const float inv = sum[j] == 0.f ? 0.f : 1.f / sum[j];
       const int token = i / p.group, head = it.w * p.group + i - token * p.group;
       E* const out = static_cast<E*>(p.out) + (row0 + token) * p.out_row + head * p.out_head + lane * kOwn;
       uint32_t w[kOwn / 2];
@@ -1367,6 +1390,7 @@ int sm_count(int* sms) {
 using namespace mf;
 
 extern "C" int64_t monofab_masked_attention_ws_bytes(int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return fail(MONOFAB_EINVAL, "masked_attention: head_dim=%d must be 64 or 128", head_dim);
   int sms = 0;
   if (int r = sm_count(&sms)) return r;
   const Grid g = grid_of(head_dim, sms);

@@ -314,3 +314,57 @@ def test_few_rows_whose_maxima_grow_and_unseen_values():
     tol = tolerance(ref, weighted, BF, 3100) + 1.5e-3 * weighted
     err = (out.double().cpu() - ref).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [[1, 1, 3], [5, 40, 33], [70, 9, 150]])
+def test_drafted_tokens_that_no_row_sees_may_hold_anything(dim, rows):
+    """Padded drafts, whose rows of the cache nobody has written: every third token is seen by none, itself included."""
+    from monoserve_b200.attention import tree_attention
+    batch = make(rows, [300, 0, 120], 32, 4, dim, 16, BF, seed=dim + rows[0], fill=float("nan"))
+    q, kc, vc, bt, start, kv = batch
+    tree = random_trees(rows, 5)
+    for r, (a, b, L) in enumerate(zip(start.tolist(), start.tolist()[1:], kv.tolist())):
+        for d in range(1, b - a, 3):
+            bit = 1 << d % 32
+            tree[a:b, d // 32] &= ~bit if bit < 1 << 31 else (1 << 31) - 1
+            tree[a + d] = 0
+            j = L - (b - a) + d
+            kc[bt[r, j // 16], j % 16] = float("nan")
+            vc[bt[r, j // 16], j % 16] = float("inf" if d % 2 else "nan")
+            q[a + d] = float("nan")
+    out = tree_attention(*on_gpu(*batch), tree.cuda())
+    padded = torch.cat([torch.arange(n) % 3 == 1 for n in rows])
+    clean = q.clone()
+    clean[padded] = 0
+    got = out.cpu()
+    past = torch.cat([torch.full((n,), int(L) > n) for n, L in zip(rows, kv)])
+    assert bool(got[padded & past].isnan().all())         # a padded row's own queries are no numbers, and it sees the past
+    assert bool((got[padded & ~past] == 0).all())         # or nothing
+    masks = tree_masks(batch, tree)
+    ref, weighted = reference(clean, kc, vc, bt, start, kv, masks)
+    err = (got.double() - ref).abs()[~padded]
+    assert bool((err <= tolerance(ref, weighted, BF, int(kv.max()))[~padded]).all())
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [20, 1], [200, 3]])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_score_that_is_no_number_shows_in_the_rows_that_see_it(rows, bad):
+    """One key at each column of a 16-column pattern, whichever way its weight is worked out; other rows are as ever."""
+    q, kc, vc, bt, start, kv = make(rows, [260, 700], 8, 1, 128, 16, BF, seed=41)
+    q = q.abs() + 0.125   # with a key of infinities: a score of infinity
+    for column in range(16):
+        key = 100 + column
+        keys = kc.clone()
+        keys[bt[0, key // 16], key % 16] = bad
+        batch = (q, keys, vc, bt, start, kv)
+        window = 260 + rows[0] // 2 - key   # seen by the first half of the request's rows; by a single one
+        window += rows[0] == 1
+        out = run_sliding(batch, window, 0).cpu()
+        sees = sliding_mask(rows[0], 260 + rows[0], window, 0)[:, key]
+        assert bool(sees.any())
+        assert bool(out[:rows[0]][sees].isnan().all())
+        good = torch.cat([~sees, torch.ones(rows[1], dtype=torch.bool)])
+        ref, weighted = reference(q, kc, vc, bt, start, kv, sliding_masks(batch, window, 0))
+        tol = tolerance(ref, weighted, BF, 800)
+        assert bool(((out.double() - ref).abs() <= tol)[good].all())

@@ -10,7 +10,7 @@ import struct
 import torch
 
 from monoserve_b200 import _C
-from monoserve_b200.attention import _HALVES, _no, _raw_stream, _refuse
+from monoserve_b200.attention import _HALVES, _no, _raw_stream, _refuse, _stream_of
 from monoserve_b200.engine import PagePool
 
 
@@ -57,7 +57,7 @@ def qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm=None, k
     for t in tensors:
         t.get_device() == index and index >= 0 or _no("all tensors must be on one CUDA device")
     if stream is not None or torch.cuda.current_device() != index:
-        with torch.cuda.device(index), torch.cuda.stream(stream):   # what is allocated in the call belongs to its stream
+        with torch.cuda.device(index), torch.cuda.stream(_stream_of(index, stream)):   # what is allocated in the call belongs to its stream
             return qk_rope(qkv, positions, slots, k_cache, v_cache, cos_sin, hq, q_norm, k_norm, eps, interleaved, q_out)
     if q_out is None:
         q_out = qkv.new_empty((T, hq, D))
@@ -87,10 +87,14 @@ class SharedPages(PagePool):
 
     def share(self, pages):
         """Another sequence holds these pages, too."""
-        _refuse(all(0 < p < self.n_pages and self.holders[p] > 0 for p in pages), "only pages that a sequence holds can be shared")
+        pages = list(pages)
+        self._held(pages)
         for p in pages:
             self.holders[p] += 1
-        return list(pages)
+        return pages
+
+    def _held(self, pages):
+        _refuse(all(0 < p < self.n_pages and self.holders[p] > 0 for p in pages), "only pages that a sequence holds can be shared")
 
     def give(self, pages):
         """A sequence lets go of these pages.  Nothing changes where one of them is not held."""
@@ -107,6 +111,7 @@ class SharedPages(PagePool):
         [(from, to)] to make for it: it shares the full pages, and gets its own copy of the one that it will go on filling."""
         full, rest = divmod(length, page_size)
         _refuse(0 <= length <= len(pages) * page_size, f"{length} tokens in {len(pages)} pages of {page_size}")
+        self._held(pages[:full + (rest > 0)])   # before a page is taken
         own = self.take(1) if rest else []
         return self.share(pages[:full]) + own, [(pages[full], p) for p in own]
 
@@ -169,9 +174,9 @@ class CachePages:
     def copy(self, src, dst, stream=None):
         """Page dst[i] takes what page src[i] holds, in all tensors.  src, dst: int32 tensors on the device, or host lists.  One page
         may go to many, but a destination may be no other pair's source or destination: lists are refused, of tensors such
-        pairs (and pages that do not exist) are left out, which check() tells."""
+        pairs (and pages that do not exist) are left out, which check() tells.  A page and itself: nothing (padding)."""
         if self._elsewhere(stream):
-            with torch.cuda.device(self.device), torch.cuda.stream(stream):
+            with torch.cuda.device(self.device), torch.cuda.stream(_stream_of(self.device.index, stream)):
                 return self.copy(src, dst)
         if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
             src, dst = list(src), list(dst)
@@ -180,6 +185,7 @@ class CachePages:
             src, dst = [s for s, _ in pairs], [d for _, d in pairs]
             len(set(dst)) == len(dst) and not set(dst) & set(src) or _no("a destination is another pair's source or destination")
             src, dst = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
+        isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) or _no("src and dst are both tensors or both lists")
         n, = self._indexes("src", src, -1)
         self._indexes("dst", dst, n)
         n <= 65535 or _no("at most 65535 pages a call")
@@ -194,7 +200,7 @@ class CachePages:
         count int32 [requests], path int32 [requests, most <= 2048], on the device.  Rows in places that do not exist stay,
         which check() tells.  Requests must not share the pages of these rows."""
         if self._elsewhere(stream):
-            with torch.cuda.device(self.device), torch.cuda.stream(stream):
+            with torch.cuda.device(self.device), torch.cuda.stream(_stream_of(self.device.index, stream)):
                 return self.accept(block_table, base, path, count)
         R, width = self._indexes("block_table", block_table, -1, -1)
         self._indexes("base", base, R)

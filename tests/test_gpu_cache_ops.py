@@ -340,3 +340,25 @@ def test_a_step_of_speculative_decoding():
     want = sliding_attention(q, kc2, vc2, bt, i32([0, 1]), i32([n + 1]), 1 << 30)
     assert torch.equal(both[0], want[0]) and torch.equal(both[1], want[0])
     assert attention_status() == 0
+
+
+def test_pages_copied_to_themselves_are_padding():
+    """Of lists and of tensors alike: as often as one likes, and beside a copy to or from the same page."""
+    from monoserve_b200.cache import CachePages
+    host = cache(2, 9, 16, 2, 64, seed=44)
+    dev = [t.cuda() for t in host]
+    pages = CachePages(dev)
+    src, dst = [0, 1, 0, 3, 5, 2, 0], [0, 2, 0, 3, 3, 2, 0]
+    for a, b in ((src, dst), [torch.tensor(t, dtype=torch.int32).cuda() for t in (src, dst)]):
+        pages.copy(a, b)
+        pages.check()
+        for t in host:
+            t[2], t[3] = t[1], t[5]
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, host))
+    out_of_range = torch.tensor([9, -1], dtype=torch.int32).cuda()
+    pages.copy(out_of_range, out_of_range)
+    with pytest.raises(RuntimeError, match="left out"):
+        pages.check()
+    for a, b in ((src, out_of_range), (out_of_range, dst)):
+        with pytest.raises(ValueError, match="both"):
+            pages.copy(a, b)

@@ -229,3 +229,29 @@ def test_shared_pages_compact():
     assert b == [moves.get(p, p) for p in b0] and c == [moves.get(p, p) for p in c0] and d == c[:2]
     assert not set(moves) & set(moves.values()) and pool.available() == 11
     assert sorted(pool.free) == list(range(9, 20)) and pool.take(1) == [9]
+
+
+def test_a_fork_of_pages_that_are_not_held_takes_none():
+    from monoserve_b200.cache import SharedPages
+    pool = SharedPages(6)
+    a = pool.take(2)
+    for pages in ([a[0], 5], [5, a[0]]):
+        with pytest.raises(ValueError, match="holds"):
+            pool.fork(pages, 20, 16)
+    assert pool.available() == 3 and sum(pool.holders) == 2
+    assert pool.fork([a[0], 5], 16, 16) == ([a[0]], [])   # the page behind the prefix does not matter
+
+
+def test_a_stream_of_another_device_is_refused():
+    from types import SimpleNamespace
+    from monoserve_b200.attention import _stream_of
+    stream = SimpleNamespace(device=torch.device("cuda", 1))
+    assert _stream_of(1, stream) is stream and _stream_of(0, None) is None
+    with pytest.raises(ValueError, match="another device"):
+        _stream_of(0, stream)
+
+
+def test_workspaces_are_for_the_head_dims_that_there_are():
+    from monoserve_b200 import _C
+    for dim in (-1, 0, 96, 256):
+        assert _C.lib.monofab_masked_attention_ws_bytes(dim) == -1 and b"head_dim" in _C.lib.monofab_last_error()

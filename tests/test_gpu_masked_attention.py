@@ -368,3 +368,16 @@ def test_a_score_that_is_no_number_shows_in_the_rows_that_see_it(rows, bad):
         ref, weighted = reference(q, kc, vc, bt, start, kv, sliding_masks(batch, window, 0))
         tol = tolerance(ref, weighted, BF, 800)
         assert bool(((out.double() - ref).abs() <= tol)[good].all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kv_len", [[4, 0, 24], [39, 1, 3], [300, 2, 4]])
+def test_trees_with_fewer_keys_than_rows(dim, kv_len):
+    """The first drafted tokens have no key: their bits say nothing, and rows that see none of the others are zeros."""
+    from monoserve_b200.attention import tree_attention
+    rows = [40, 2, 4]
+    q, kc, vc, bt, start, _ = make(rows, [300, 0, 20], 32, 4, dim, 16, BF, seed=77)
+    for empty in (False, True):
+        tree = random_trees(rows, 78, empty)
+        batch = (q, kc, vc, bt, start, torch.tensor(kv_len, dtype=torch.int32))
+        check(tree_attention(*on_gpu(*batch), tree.cuda()), batch, tree_masks(batch, tree))

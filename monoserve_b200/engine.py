@@ -58,10 +58,13 @@ class PagePool:
         return len(self.free)
 
     def take(self, n):
+        if n < 0:
+            raise ValueError(f"{n} KV pages wanted")
         if n > len(self.free):
             raise MemoryError(f"{n} KV pages wanted, {len(self.free)} free")
-        out = self.free[-n:][::-1]
-        del self.free[-n:]
+        left = len(self.free) - n   # a positive index: [-n:] is the whole list where n is 0
+        out = self.free[left:][::-1]
+        del self.free[left:]
         return out
 
     def give(self, pages):

@@ -33,6 +33,21 @@ def test_page_pool_never_hands_out_the_sink_or_a_page_twice():
     assert sorted(pool.take(4)) == sorted(a)
 
 
+def test_no_pages_wanted_are_none_and_fewer_are_refused():
+    from monoserve_b200.cache import SharedPages
+    for pool in (PagePool(6), SharedPages(6)):
+        held = pool.take(2)
+        for n in (0, -1, -3):
+            if n == 0:
+                assert pool.take(n) == []
+            else:
+                with pytest.raises(ValueError, match="wanted"):
+                    pool.take(n)
+            assert pool.free == [5, 4, 3] and held == [1, 2]
+        assert getattr(pool, "holders", [0, 1, 1, 0, 0, 0]) == [0, 1, 1, 0, 0, 0]
+        assert pool.take(3) == [3, 4, 5] and pool.take(0) == []
+
+
 def test_search_planner_splits_the_workers_between_the_lanes():
     """The engine's planner: the control plane's plan search over the committed B200 calibration gives the decode
     lane a share that grows with its batch and shrinks when the prefill pass grows; one lane alone needs no split."""

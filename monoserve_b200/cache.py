@@ -98,6 +98,7 @@ class SharedPages(PagePool):
 
     def give(self, pages):
         """A sequence lets go of these pages.  Nothing changes where one of them is not held."""
+        pages = list(pages)   # gone through twice
         left = {}
         for p in pages:
             _refuse(0 < p < self.n_pages and left.setdefault(p, self.holders[p]) > 0, f"page {p} is held by no sequence")

@@ -255,3 +255,11 @@ def test_workspaces_are_for_the_head_dims_that_there_are():
     from monoserve_b200 import _C
     for dim in (-1, 0, 96, 256):
         assert _C.lib.monofab_masked_attention_ws_bytes(dim) == -1 and b"head_dim" in _C.lib.monofab_last_error()
+
+
+def test_pages_given_by_an_iterator_are_free_again():
+    from monoserve_b200.cache import SharedPages
+    pool = SharedPages(6)
+    a = pool.take(3)
+    pool.give(p for p in a)
+    assert sorted(pool.free) == [1, 2, 3, 4, 5] and not any(pool.holders)

@@ -120,7 +120,9 @@ class SharedPages(PagePool):
         """Moves held pages to the lowest numbers.  sequences: lists of pages, all that are held; their entries are
         replaced.  Returns the copies [(from, to)] to make before anybody reads the new pages."""
         seen = [0] * self.n_pages
+        sequences = list(sequences)   # gone through twice
         for pages in sequences:
+            _refuse(hasattr(pages, "__setitem__"), "compact replaces the entries of the sequences' lists")
             for p in pages:
                 _refuse(0 < p < self.n_pages, f"page {p} is no page of the pool")
                 seen[p] += 1

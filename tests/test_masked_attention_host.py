@@ -263,3 +263,15 @@ def test_pages_given_by_an_iterator_are_free_again():
     a = pool.take(3)
     pool.give(p for p in a)
     assert sorted(pool.free) == [1, 2, 3, 4, 5] and not any(pool.holders)
+
+
+def test_compact_takes_an_iterator_and_refuses_what_it_cannot_replace():
+    from monoserve_b200.cache import SharedPages
+    pool = SharedPages(9)
+    a, b, c = pool.take(3), pool.take(2), pool.take(2)
+    pool.give(a)
+    with pytest.raises(ValueError, match="lists"):
+        pool.compact([b, tuple(c)])
+    assert b == [4, 5] and pool.holders == [0, 0, 0, 0, 1, 1, 1, 1, 0]   # nothing has changed
+    assert pool.compact(s for s in [b, c]) == [(5, 1), (6, 2), (7, 3)]
+    assert b == [4, 1] and c == [2, 3] and pool.holders == [0, 1, 1, 1, 1, 0, 0, 0, 0]

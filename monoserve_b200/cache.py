@@ -216,8 +216,11 @@ class CachePages:
             _C.check(rc)
 
     def check(self):
-        """Raises if a copy or an accept since the last check left something out.  Waits for the device."""
+        """Raises if a copy or an accept since the last check left something out, on whatever stream it was called or replayed.
+        Waits for the device (and so for a resident fabric to stop)."""
+        torch.cuda.synchronize(self.device)
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
+            torch.cuda.synchronize(self.device)   # the bits of a call on another stream come behind this
             raise RuntimeError(f"monofab: pages or rows were left out, status {bits}")

@@ -362,3 +362,29 @@ def test_pages_copied_to_themselves_are_padding():
     for a, b in ((src, out_of_range), (out_of_range, dst)):
         with pytest.raises(ValueError, match="both"):
             pages.copy(a, b)
+
+
+def test_a_check_waits_for_calls_on_other_streams():
+    """The side stream is busy when its call is made, so that the call has not run when check() is asked."""
+    from monoserve_b200.cache import CachePages
+    pages = CachePages([t.cuda() for t in cache(1, 9, 16, 2, 64, seed=45)])
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()   # noqa: E731
+    missing, page, one, zero, table = i32([9]), i32([2]), i32([1]), i32([0]), i32([[1, 9]])
+    far = i32([[20]])   # row 20 of the table's pages is in page 9
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pages.copy(missing, page)
+
+    def replayed():
+        with torch.cuda.stream(side):
+            graph.replay()
+
+    torch.cuda.synchronize()
+    for call in (lambda: pages.copy(missing, page, stream=side), lambda: pages.accept(table, zero, far, one, stream=side), replayed):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)   # cycles: some 50 ms
+        call()
+        with pytest.raises(RuntimeError, match="left out"):
+            pages.check()
+        pages.check()

@@ -4,7 +4,8 @@
 // o_i = sum_j p_ij v_j / sum_j p_ij over the keys j that row i sees, p_ij = 2^(c s_ij - m_i), s = q k, c = scale log2(e), in one
 // pass over the keys in tiles of 128. m_i is a reference that all of a row's weights share: the first maximum, moved only when a later
 // one passes it by more than 2^8, and then the sums so far are scaled. Scores, sums and outputs are in 32 bits; a weight is rounded
-// once, to the type of V, for the product.
+// once, to the type of V, for the product: its matrix instruction wants both operands alike. Weights of fp16 are 2^7 times as large, so
+// that they use the type's range upwards as well (below 2^16) and those far below the reference are not lost: steps of 2^-31 of it.
 //
 //   * An item is (request, block of query tokens, KV head); a row of the matrix products is a (token, query head of the group) pair,
 //     so a K or V tile is read once for all of them. A CTA has two streams of 128 rows, each with scores S (128 columns of TMEM), the
@@ -65,7 +66,7 @@ constexpr int kSlotRows = 2 * kTile;
 constexpr int kMaxRequests = 16384;
 constexpr int kFewRows = 16, kFewBytes = 2 * kFewRows * 128;   // kFewBytes: weights of such a stream, two times 64 keys of a row in 128 bytes
 constexpr unsigned long long kWaitNs = 2000000000ull;
-constexpr float kSlack = 8.f;
+constexpr float kSlack = 8.f;       // powers of two by which a weight may pass that of its reference
 constexpr int kByFma = 8;           // weights of 32 worked out by multiplications
 
 // Where a call that names no status word leaves its bits.
@@ -273,6 +274,7 @@ struct Half2;
 template <>
 struct Half2<__nv_bfloat16> {
   static constexpr uint32_t kFormat = 1;
+  static constexpr float kLift = 0.f;   // weights are 2^kLift times p_ij, sums and outputs alike; bf16 has the exponents of fp32
   // 2^x on [-1/2, 1/2] with the least relative error of its degree, 7.5e-5: a fiftieth of the rounding to bf16 that follows
   static __device__ __forceinline__ Pair power(Pair f) {
     Pair y = pair_of(0.05517166852951f, 0.05517166852951f);
@@ -288,6 +290,7 @@ struct Half2<__nv_bfloat16> {
 template <>
 struct Half2<__half> {
   static constexpr uint32_t kFormat = 0;
+  static constexpr float kLift = 7.f;   // with kSlack below 2^16
   // one degree more, 2.6e-6, for fp16's smaller rounding
   static __device__ __forceinline__ Pair power(Pair f) {
     Pair y = pair_of(0.00957010220736f, 0.00957010220736f);
@@ -301,6 +304,7 @@ struct Half2<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 };
+static_assert(Half2<__half>::kLift + kSlack < 16.f, "weights are finite in fp16");
 template <class E>
 __host__ __device__ constexpr uint32_t idesc_of(int n) {   // fp32 accumulators, M = 128
   return (1u << 4) | (Half2<E>::kFormat << 7) | (Half2<E>::kFormat << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
@@ -882,7 +886,7 @@ __device__ bool softmax_few(const Params& p, Shared& sh, uint8_t* q_mem, const R
         store_tmem_wait();
       }
       held = moved;
-      const float shift = held == -INFINITY ? 0.f : held;
+      const float shift = held == -INFINITY ? 0.f : held - Half2<E>::kLift;
 #pragma unroll
       for (int i = 0; i < N; ++i) m[i] = __shfl_sync(0xffffffffu, shift, i);
     }
@@ -1077,7 +1081,7 @@ __device__ void softmax(const Params& p, Shared& sh, uint8_t* q_mem, int wg) {
         }
       }
       begun = true;
-      const float shift = m == -INFINITY ? 0.f : -m;
+      const float shift = m == -INFINITY ? 0.f : Half2<E>::kLift == 0.f ? -m : Half2<E>::kLift - m;
       Pair sum = 0ull;
 #pragma unroll 1
       for (int c = 0; c < kTile; c += 32) {

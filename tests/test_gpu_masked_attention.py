@@ -381,3 +381,42 @@ def test_trees_with_fewer_keys_than_rows(dim, kv_len):
         tree = random_trees(rows, 78, empty)
         batch = (q, kc, vc, bt, start, torch.tensor(kv_len, dtype=torch.int32))
         check(tree_attention(*on_gpu(*batch), tree.cuda()), batch, tree_masks(batch, tree))
+
+
+def far_below_the_reference(out, weighted, keys_per_one):
+    """As tolerance() for fp16, whose weights have steps of 2^-31 of their reference at worst: half of that for each key, times
+    keys_per_one, the keys times |v| for each whole unit of the sum of weights."""
+    half = torch.finfo(FP).eps / 2
+    return half * out.abs() + (half + 3e-4) * weighted + keys_per_one * 2.0 ** -32 + 2.0 ** -25
+
+
+@pytest.mark.parametrize("dim,hq,rows", [(128, 8, [1]), (128, 8, [5]), (128, 8, [40]), (64, 8, [1]), (64, 2, [200])])
+def test_fp16_weights_far_below_the_largest_count(dim, hq, rows):
+    """One key of 64 has nearly all the weight and no value; 63 others have 2^-26 of it each and large values, which are the output.
+    As columns and as rows of the products, of one stream's rows and of two."""
+    q, kc, vc, bt, start, kv = make(rows, [640], hq, 1, dim, 16, FP, seed=51)
+    q.zero_(), kc.zero_(), vc.fill_(1000.0)
+    q[:, :, 0] = 1
+    for j in range(0, int(kv[0]), 64):
+        kc[bt[0, j // 16], j % 16, :, 0] = 18.0   # 18 log2(e) = 25.97
+        vc[bt[0, j // 16], j % 16] = 0
+    batch = (q, kc, vc, bt, start, kv)
+    out = run_sliding(batch, 1 << 30, 0, scale=1.0).double().cpu()
+    ref, weighted = reference(*batch, sliding_masks(batch, 1 << 30, 0), scale=1.0)
+    assert float(ref.min()) > 8e-4
+    err = (out - ref).abs()
+    assert bool((err <= far_below_the_reference(ref, weighted, 64 * 1000)).all()), float((err / ref).max())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_fp16_weights_of_ragged_batches(dim, hq, hkv):
+    """The sum of a row's weights is one at least in units of its largest, which is its reference or above it."""
+    batch = make([1, 5, 0, 33, 130, 1], [0, 700, 50, 3, 260, 2049], hq, hkv, dim, 16, FP, seed=hq + dim + 52)
+    for window, sinks in ((7, 3), (500, 17), (1 << 30, 0)):
+        out = run_sliding(batch, window, sinks, scale=0.5).double().cpu()   # peaked: scores of several times the usual ones
+        ref, weighted = reference(*batch, sliding_masks(batch, window, sinks), scale=0.5)
+        # a weight's exponent is off by 128 * 2^-24 * 128 * 0.5 = 4.9e-4 at most and its power of two by 2^-13; so is the sum
+        tol = far_below_the_reference(ref, weighted, int(batch[5].max()) * 6) + 2 * 6.2e-4 * weighted
+        err = (out - ref).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())

@@ -133,13 +133,17 @@ __device__ __forceinline__ Span span_of(const Params& p, const Request& q, int b
   s.hi = max(0, min(there, s.pos0 + s.tokens));
   const int lo = static_cast<int>(max(0ll, static_cast<long long>(s.pos0) - p.window + 1));
   s.near = min(min(p.sinks, s.hi), lo);
+  if (lo >= there) {   // no key of the window is there: places are keys, and none of them is past 2^30
+    s.lo = s.hi = s.near;
+    return s;
+  }
   const int split = (s.near + p.page - 1) / p.page * p.page, from = lo / p.page * p.page;
   if (split < from) {
     s.split = split;
     s.shift = from - split;
   }
   s.lo = lo - s.shift;
-  s.hi = max(s.near, s.hi - s.shift);   // below lo where the window has no key that is there
+  s.hi = max(s.near, s.hi - s.shift);
   return s;
 }
 

@@ -420,3 +420,20 @@ def test_fp16_weights_of_ragged_batches(dim, hq, hkv):
         tol = far_below_the_reference(ref, weighted, int(batch[5].max()) * 6) + 2 * 6.2e-4 * weighted
         err = (out - ref).abs()
         assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [[1], [10], [40]])
+@pytest.mark.parametrize("window", [1, 20, 2000, (1 << 31) - 700, (1 << 31) - 1])
+@pytest.mark.parametrize("sinks", [0, 5, 300])
+def test_positions_up_to_the_largest(dim, rows, window, sinks):
+    """As many keys as an int32 can say, of which the block table has the first 640: most windows lie behind all of them."""
+    q, kc, vc, bt, start, _ = make(rows, [640 - rows[0]], 8, 1, dim, 16, BF, seed=54)
+    L = (1 << 31) - 1
+    p, j = torch.arange(L - rows[0], L)[:, None], torch.arange(640)[None]
+    mask = (j > p - window) | (j < sinks)
+    batch = (q, kc, vc, bt, start, torch.tensor([L], dtype=torch.int32))
+    out = run_sliding(batch, window, sinks)
+    ref, weighted = reference(*batch, [mask])
+    err = (out.double().cpu() - ref).abs()
+    assert bool((err <= tolerance(ref, weighted, BF, 640)).all()), float(err.max())

@@ -165,6 +165,15 @@ def _stream_of(index, stream):
     return stream
 
 
+def _apart(row, rows, head, heads, D):
+    """Whether `rows` by `heads` runs of D values, at these strides, have no value in common."""
+    (near, n), (far, m) = sorted([(row, rows), (head, heads)])
+    if near >= D and far >= (n - 1) * near + D:   # one inside the other, as nearly all are
+        return True
+    # else two runs lie a * near - b * far apart, a < n, b < m: the nearest a of each b, those of b = 0 one step
+    return (n == 1 or near >= D) and all(abs(min(n - 1, max(0, a)) * near - b * far) >= D for b in range(1, m) for a in (b * far // near, b * far // near + 1))
+
+
 @functools.lru_cache(maxsize=None)
 def _masked_ws_bytes(device_index, head_dim):
     n = _C.lib.monofab_masked_attention_ws_bytes(head_dim)
@@ -213,6 +222,7 @@ def _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
         T == 0 or (last == 1 and (row | head) % 8 == 0 and row > 0 and head > 0 and t.data_ptr() % 16 == 0) or \
             _no("the heads of q and out must be contiguous and start at multiples of 16 bytes")
         if t is out:
+            T == 0 or _apart(row, T, head, hq, D) or _no("rows and heads of out must not overlap")
             out_strides = row, head
     index >= 0 and here and k_cache.get_device() == index and v_cache.get_device() == index and \
         (out is None or out.get_device() == index) and (status is None or status.get_device() == index) or _no("all tensors must be on one CUDA device")
@@ -243,7 +253,7 @@ def sliding_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     [pages, page_size, hkv, D]; block_table int32 [requests, stride]; q_start int32 [requests + 1]: request r's rows are
     q_start[r] .. q_start[r + 1] - 1; kv_len int32 [requests]: its keys, those of its rows the last of them.  The lengths are read
     on the device: a call captured in a CUDA graph can be replayed with others.  Returns [T, hq, D] (`out`, which may be q
-    itself): rows that see no key are zeros, rows of no request keep what they hold (are undefined in a new tensor).
+    itself, or else shares no memory with it): rows that see no key are zeros, rows of no request keep what they hold (are undefined in a new tensor).
     A bounded wait that ran out is reported in `status` (int32 on the device), or to attention_status().  Values that some row
     of a request sees must be finite; what none sees may hold anything.  A score that is infinite or no number makes the rows
     that see it NaN.  At most 16384 requests."""

@@ -275,3 +275,26 @@ def test_compact_takes_an_iterator_and_refuses_what_it_cannot_replace():
     assert b == [4, 5] and pool.holders == [0, 0, 0, 0, 1, 1, 1, 1, 0]   # nothing has changed
     assert pool.compact(s for s in [b, c]) == [(5, 1), (6, 2), (7, 3)]
     assert b == [4, 1] and c == [2, 3] and pool.holders == [0, 1, 1, 1, 1, 0, 0, 0, 0]
+
+
+def test_an_out_whose_rows_overlap_is_refused():
+    """Where several rows or heads share memory, which of their results stays would be left to chance."""
+    from monoserve_b200.attention import _apart, sliding_attention
+
+    def call(row, head, T=4, hq=8, buffer=torch.zeros(1 << 16, dtype=BF)):
+        sliding_attention(**{**attention_args(T=T, hq=hq), "out": torch.as_strided(buffer, (T, hq, 128), (row, head, 1))}, window=5)
+
+    for row, head in ((64, 4096), (1024, 64), (512, 128), (256, 512), (8, 8), (128, 128), (384, 256)):
+        with pytest.raises(ValueError, match="must not overlap"):
+            call(row, head)
+    # apart: contiguous, wider, heads first, interleaved; single rows and heads at any stride
+    for row, head in ((1024, 128), (2048, 136), (128, 512), (256, 1024), (1536, 128)):
+        with pytest.raises(ValueError, match="one CUDA device"):
+            call(row, head)
+    with pytest.raises(ValueError, match="one CUDA device"):
+        call(8, 128, T=1)
+    for n, m, D in ((1, 1, 8), (1, 5, 8), (4, 3, 8), (5, 5, 16), (7, 2, 8)):   # against every pair of runs
+        for row in range(8, 160, 8):
+            for head in range(8, 160, 8):
+                runs = sorted(i * row + j * head for i in range(n) for j in range(m))
+                assert _apart(row, n, head, m, D) == all(y - x >= D for x, y in zip(runs, runs[1:])), (n, m, D, row, head)

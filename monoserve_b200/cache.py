@@ -155,7 +155,8 @@ class CachePages:
         self.row_bytes = t0.shape[2] * t0.shape[3] * t0.element_size()
         _refuse(self.n_pages >= 1 and self.page_size >= 1 and self.row_bytes >= 16 and self.row_bytes % 16 == 0 and all(t.data_ptr() % 16 == 0 for t in tensors),
                 "rows of a cache tensor must be multiples of 16 bytes")
-        _refuse(len(tensors) <= 65535 and len({t.data_ptr() for t in tensors}) == len(tensors), "at most 65535 cache tensors, each of them once")
+        at, size = sorted(t.data_ptr() for t in tensors), t0.numel() * t0.element_size()
+        _refuse(len(tensors) <= 65535 and all(b - a >= size for a, b in zip(at, at[1:])), "at most 65535 cache tensors, each of them once and in memory of its own")
         _refuse(t0.is_cuda, "cache tensors must be on a CUDA device")
         self.tensors, self.device = tensors, t0.device
         self._table = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64).to(self.device)

@@ -298,3 +298,13 @@ def test_an_out_whose_rows_overlap_is_refused():
             for head in range(8, 160, 8):
                 runs = sorted(i * row + j * head for i in range(n) for j in range(m))
                 assert _apart(row, n, head, m, D) == all(y - x >= D for x, y in zip(runs, runs[1:])), (n, m, D, row, head)
+
+
+def test_cache_tensors_that_share_pages_are_refused():
+    from monoserve_b200.cache import CachePages
+    t = torch.zeros(10, 16, 2, 64, dtype=BF)
+    for tensors in ([t[:4], t[2:6]], [t[6:], t[:4], t[3:7]], [t[:4], t[:4]]):
+        with pytest.raises(ValueError, match="each of them once"):
+            CachePages(tensors)
+    with pytest.raises(ValueError, match="CUDA device"):
+        CachePages([t[6:], t[:4]])

@@ -141,7 +141,9 @@ int monofab_attention(const void* q, const void* k_cache, const void* v_cache, v
  *                  tree[row][d / 32]; those from 32 * words on have none.
  * out = sum_j softmax_j(scale q k_j) v_j; a row that sees no key is zeros.  Rows of no request keep what they hold.
  * Values that some row of a request sees must be finite, also for that request's rows that do not see them; what no row sees
- * may hold anything.  A row that sees a score that is infinite or no number is NaN.  At most 16384 requests a call.
+ * may hold anything.  A row that sees a score of plus infinity or no number is NaN; minus infinity has weight zero, and a row
+ * whose scores are all that is zeros.  Scores, sums and outputs are in 32 bits; a weight is rounded once, to the type of V, for
+ * its product (the sum takes it unrounded).  At most 16384 requests a call.
  * Keys past the block table (kv_len > bt_stride * page_size) are not there; a page number outside [0, n_pages) reads as
  * zeros; q_start is taken as ascending within [0, tokens], and a request that it gives no rows has none. */
 typedef struct {

@@ -255,8 +255,9 @@ def sliding_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     on the device: a call captured in a CUDA graph can be replayed with others.  Returns [T, hq, D] (`out`, which may be q
     itself, or else shares no memory with it): rows that see no key are zeros, rows of no request keep what they hold (are undefined in a new tensor).
     A bounded wait that ran out is reported in `status` (int32 on the device), or to attention_status().  Values that some row
-    of a request sees must be finite; what none sees may hold anything.  A score that is infinite or no number makes the rows
-    that see it NaN.  At most 16384 requests."""
+    of a request sees must be finite; what none sees may hold anything.  A score of plus infinity or no number makes the rows
+    that see it NaN; minus infinity has weight zero, and rows whose scores are all that are zeros.  Scores, sums and outputs are in
+    32 bits; a weight is rounded once, to the type of V, for its product.  At most 16384 requests."""
     return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, int(window), int(sinks), None, scale, out, stream, status)
 
 

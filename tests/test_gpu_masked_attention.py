@@ -437,3 +437,20 @@ def test_positions_up_to_the_largest(dim, rows, window, sinks):
     ref, weighted = reference(*batch, [mask])
     err = (out.double().cpu() - ref).abs()
     assert bool((err <= tolerance(ref, weighted, BF, 640)).all()), float(err.max())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [[1, 1], [9, 1], [20, 1], [200, 3]])
+def test_a_score_of_minus_infinity_has_no_weight(dim, rows):
+    """As the formula says: the power of minus infinity is zero. Rows whose scores are all that are zeros, as those that see no key."""
+    n = rows[0]
+    q, kc, vc, bt, start, kv = make(rows, [260, 700], 8, 1, dim, 16, BF, seed=55)
+    q = q.abs() + 0.125
+    for j in range(260 - 10, 260 + (n + 1) // 2):   # keys in front of the rows, and of the first half of them
+        kc[bt[0, j // 16], j % 16] = -float("inf")
+    batch = (q, kc, vc, bt, start, kv)
+    for window, sinks in ((8, 0), (8, 3), (1 << 30, 0)):
+        out = run_sliding(batch, window, sinks)
+        check(out, batch, sliding_masks(batch, window, sinks))
+        if (window, sinks) == (8, 0):
+            assert bool((out[:(n + 1) // 2] == 0).all())

@@ -439,6 +439,18 @@ def test_positions_up_to_the_largest(dim, rows, window, sinks):
     assert bool((err <= tolerance(ref, weighted, BF, 640)).all()), float(err.max())
 
 
+NO_WINDOW = (1 << 31) - 1   # the largest numbers that a call takes
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [[1, 1, 1, 1], [1, 20, 0, 150]])
+@pytest.mark.parametrize("window,sinks", [(NO_WINDOW, 0), (NO_WINDOW, NO_WINDOW), (1, NO_WINDOW), (100, NO_WINDOW), (130, 200)])
+def test_the_largest_windows_and_sinks(dim, rows, window, sinks):
+    """As columns (dim 128, single tokens) and as rows of the products."""
+    batch = make(rows, [700, 129, 5, 0], 32, 4, dim, 16, BF, seed=53)
+    check(run_sliding(batch, window, sinks), batch, sliding_masks(batch, window, sinks))
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("rows", [[1, 1], [9, 1], [20, 1], [200, 3]])
 def test_a_score_of_minus_infinity_has_no_weight(dim, rows):
@@ -454,3 +466,24 @@ def test_a_score_of_minus_infinity_has_no_weight(dim, rows):
         check(out, batch, sliding_masks(batch, window, sinks))
         if (window, sinks) == (8, 0):
             assert bool((out[:(n + 1) // 2] == 0).all())
+
+
+def test_every_ancestor_of_a_drafted_token_counts():
+    """A tree behind a short past, within a bound for each element that no other tree's result would keep: any one bit of the
+    oracle's masks turned over shows in its row."""
+    from monoserve_b200.attention import attention_status, tree_attention, tree_bits
+    batch = make([7], [37], 8, 2, 128, 16, BF, seed=56)
+    tree = tree_bits([-1, 0, 0, 1, 2, 2, 5])
+    out = tree_attention(*on_gpu(*batch), tree.cuda()).double().cpu()
+    assert attention_status() == 0
+
+    def off(words):
+        ref, weighted = reference(*batch, tree_masks(batch, words))
+        return ((out - ref).abs() / tolerance(ref, weighted, BF, 44)).amax((1, 2))
+
+    assert bool((off(tree) <= 1).all())
+    for row in range(7):
+        for d in range(7):
+            other = tree.clone()
+            other[row, 0] ^= 1 << d
+            assert float(off(other)[row]) > 1, (row, d)

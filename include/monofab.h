@@ -165,7 +165,8 @@ typedef struct {
   float scale;                 /* of the scores, positive */
   int32_t reserved;
 } monofab_masked_attention_args;
-/* Bytes of a call's workspace on the current device, or a negative error code. */
+/* Bytes of a call's workspace on the current device, or a negative error code: two parts of 256 rows for each SM whatever the
+ * call's sizes, 39 MB on 148 SMs at head_dim 128 and 20 MB at 64. */
 int64_t monofab_masked_attention_ws_bytes(int head_dim);
 int monofab_masked_attention(const monofab_masked_attention_args* args, void* stream);
 /* The current device's own status word of these calls, read (the device is synchronised) and cleared. */

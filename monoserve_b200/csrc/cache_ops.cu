@@ -4,7 +4,7 @@
 //
 // A cache tensor is [pages][page size][kv heads][head dim], 16-bit values; a slot is page * page size + row in the page.
 // All of this is bound by HBM or, for a few rows, by the latency of one launch: every kernel keeps several 16-byte accesses a
-// thread in flight and touches each byte once.
+// thread in flight and touches each byte of the caches once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -209,6 +209,8 @@ constexpr int kCopyThreads = 256, kCopyLoads = 4, kCopyBytes = kCopyThreads * kC
 // Block (chunk of a page, tensor, pair): 131 pages of 16 KB in 96 tensors take 66 us, 6.2 TB/s. Whether the pair may be copied is looked at first, in every block alike:
 // its destination may be no other pair's source or destination, and its source no other pair's destination - copies run side
 // by side, and either would make the result depend on their order. A page to itself is nothing to do, and in nobody's way.
+// Every block reads both lists for that, which grows with the square of the pairs: 4096 pairs of 16 KB are still at HBM's rate (1946 us,
+// 6.6 TB/s), of 16384 the lists take half the time (17.2 ms, 3.0 TB/s), and beside pages of 1 KB those of 4096 do most of the work (0.6 TB/s).
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_constant__ PageCopyParams p) {
   chain_release();
   chain_wait();
@@ -254,7 +256,8 @@ constexpr int kAcceptThreads = 256, kAcceptRows = 8;   // rows a thread holds at
 // anywhere among the drafts, whatever it overwrites. The slice is as wide as lets the block's threads hold all rows.
 // What bounds it is the chain count, path, table, row: it is gone through once for a group of tensors, and the next
 // tensor's rows are on their way while the last one's are written. (64 requests, 96 tensors, 4 moved rows of 1 KB each: 15.7 us,
-// 3.5 TB/s; a block for each tensor: 42.7.)
+// 3.5 TB/s; a block for each tensor: 42.7. With 38, 63 and 126 registers 6, 4 and 2 blocks of the three forms fit on an SM: these 1280
+// blocks of the middle one go through the chain in three rounds.)
 template <int kRows>
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptParams p) {
   chain_release();
@@ -414,7 +417,7 @@ extern "C" int monofab_accept_rows(const uint64_t* tensors, int n_tensors, const
   p.lanes = 1;
   while (2 * p.lanes <= kAcceptThreads && 2 * p.lanes * most <= kAcceptThreads * kAcceptRows && p.lanes < p.pieces) p.lanes *= 2;
   const int slices = (p.pieces + p.lanes - 1) / p.lanes, rows = (most * p.lanes + kAcceptThreads - 1) / kAcceptThreads;
-  // as many tensors a block as leave every SM its blocks
+  // up to 16 tensors a block, as many as leave eight blocks for each SM (not all of them there at once: see the kernel)
   int blocks = 0;
   MF_CUDA(resident_blocks(&blocks, 8));
   const long long all = static_cast<long long>(slices) * n_tensors * requests;

@@ -1363,7 +1363,7 @@ struct Grid {
   int ctas;
   size_t o_bytes, ml_bytes, meta_bytes;
 };
-// One CTA per SM, or per tile of the largest call that the sizes allow.
+// One CTA per SM and the workspace of all of them, whatever the call: how much there is to do stands in lengths on the device.
 Grid grid_of(int head_dim, int sms) {
   Grid g;
   g.ctas = sms;
@@ -1476,7 +1476,9 @@ extern "C" int monofab_masked_attention(const monofab_masked_attention_args* a, 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Batches of single tokens and the like (by the mean of their rows: what the host knows) take the kernel that also has a form for items
   // of few rows. 128 single tokens over 843 MB, long runs: 153 us, without the form 177 (at the card's power limit: 128 rows of products
-  // for eight that are there); but its code alone, unused, made window prompts 157 -> 162.
+  // for eight that are there); but its code alone, unused, makes prompts 114 -> 121. The mean is a rough rule: 127 single tokens beside a
+  // portion of 512 rows (1.14 GB) take 245 us without the form, 230 with it. Head dimension 64 has no such form: 128 single tokens
+  // over 571 MB take 175 us, 3.3 TB/s.
   const bool few = static_cast<int64_t>(a->tokens) * group <= static_cast<int64_t>(a->requests) * kFewRows;
   auto go = [&](auto e) {
     using E = decltype(e);

@@ -143,7 +143,8 @@ int monofab_attention(const void* q, const void* k_cache, const void* v_cache, v
  * Values that some row of a request sees must be finite, also for that request's rows that do not see them; what no row sees
  * may hold anything.  A row that sees a score of plus infinity or no number is NaN; minus infinity has weight zero, and a row
  * whose scores are all that is zeros.  Scores, sums and outputs are in 32 bits; a weight is rounded once, to the type of V, for
- * its product (the sum takes it unrounded).  At most 16384 requests a call.
+ * its product (the sum takes it unrounded).  Scores may be 10^7 in magnitude with fp16 values, 5 10^8 with bf16: a step of a
+ * larger one is more than the weights' type has room for.  At most 16384 requests a call.
  * Keys past the block table (kv_len > bt_stride * page_size) are not there; a page number outside [0, n_pages) reads as
  * zeros; q_start is taken as ascending within [0, tokens], and a request that it gives no rows has none. */
 typedef struct {

@@ -257,7 +257,7 @@ def sliding_attention(q, k_cache, v_cache, block_table, q_start, kv_len, window,
     A bounded wait that ran out is reported in `status` (int32 on the device), or to attention_status().  Values that some row
     of a request sees must be finite; what none sees may hold anything.  A score of plus infinity or no number makes the rows
     that see it NaN; minus infinity has weight zero, and rows whose scores are all that are zeros.  Scores, sums and outputs are in
-    32 bits; a weight is rounded once, to the type of V, for its product.  At most 16384 requests."""
+    32 bits; a weight is rounded once, to the type of V, for its product.  Scores may be 1e7 in magnitude (bf16: 5e8).  At most 16384 requests."""
     return _masked_attention(q, k_cache, v_cache, block_table, q_start, kv_len, int(window), int(sinks), None, scale, out, stream, status)
 
 

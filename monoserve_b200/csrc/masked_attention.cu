@@ -6,6 +6,7 @@
 // one passes it by more than 2^8, and then the sums so far are scaled. Scores, sums and outputs are in 32 bits; a weight is rounded
 // once, to the type of V, for the product: its matrix instruction wants both operands alike. Weights of fp16 are 2^7 times as large, so
 // that they use the type's range upwards as well (below 2^16) and those far below the reference are not lost: steps of 2^-31 of it.
+// All of a row's weights share the rounding of m_i, half a step of it: harmless while 2^8 times that is in the type (c s up to 2^24 in fp16).
 //
 //   * An item is (request, block of query tokens, KV head); a row of the matrix products is a (token, query head of the group) pair,
 //     so a K or V tile is read once for all of them. A CTA has two streams of 128 rows, each with scores S (128 columns of TMEM), the
@@ -84,7 +85,7 @@ struct Params {
   float2* ws_ml;          // [2 x CTAs][256]
   int4* ws_meta;          // [CTAs][2]
   long long out_row, out_head;
-  int tokens, requests, hkv, group, page, n_pages, bt_stride, words, window, sinks;
+  int tokens, requests, hkv, group, page, bt_stride, words, window, sinks;
   int per_stream;         // query tokens of a stream's 128 rows
   float scale_log2;
 };
@@ -1467,7 +1468,6 @@ extern "C" int monofab_masked_attention(const monofab_masked_attention_args* a, 
   p.hkv = a->hkv;
   p.group = group;
   p.page = a->page_size;
-  p.n_pages = a->n_pages;
   p.bt_stride = a->bt_stride;
   p.words = a->words;
   p.window = a->window;

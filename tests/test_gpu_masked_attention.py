@@ -487,3 +487,78 @@ def test_every_ancestor_of_a_drafted_token_counts():
             other = tree.clone()
             other[row, 0] ^= 1 << d
             assert float(off(other)[row]) > 1, (row, d)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [9, 40, 1]])
+def test_pages_that_do_not_exist_read_as_zeros(dim, rows):
+    from monoserve_b200.attention import tree_attention
+    q, kc, vc, bt, start, kv = make(rows, [300, 500, 90], 32, 4, dim, 16, BF, seed=57)
+    n = kc.shape[0]
+    bad = bt.clone()
+    for r, column, page in ((0, 1, -1), (0, 12, n), (0, 18, n + 1000), (1, 0, -1000), (1, 20, n), (1, 31, -1), (2, 5, n)):
+        bad[r, column] = page
+    zeros = torch.where((bad < 0) | (bad >= n), n, bad)   # the oracle has a page of zeros for them
+    kz, vz = (torch.cat([t, torch.zeros_like(t[:1])]) for t in (kc, vc))
+    oracle = (q, kz, vz, zeros, start, kv)
+    for window, sinks in ((1 << 30, 0), (150, 20)):
+        check(run_sliding((q, kc, vc, bad, start, kv), window, sinks), oracle, sliding_masks(oracle, window, sinks))
+    tree = random_trees(rows, 58)
+    check(tree_attention(*on_gpu(q, kc, vc, bad, start, kv), tree.cuda()), oracle, tree_masks(oracle, tree))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_row_starts_that_are_no_ascending_places(dim):
+    """Taken within [0, tokens]; a request that ends in front of its begin has no rows, and rows of nobody stay."""
+    from monoserve_b200.attention import sliding_attention
+    q, kc, vc, bt, _, kv = make([3, 0, 7, 0, 4], [90, 200, 0, 30, 500], 32, 4, dim, 16, BF, seed=59)
+    T = len(q)
+    said = torch.tensor([-5, 3, 2, 10, 9, 1 << 30], dtype=torch.int32)
+    taken = [(0, 3), (3, 3), (2, 10), (10, 10), (9, T)]
+    out = torch.full_like(q, 5.0).cuda()
+    # requests 0 and 2 say rows 2 both, 2 and 4 row 9: the test looks at the others
+    sliding_attention(*on_gpu(q, kc, vc, bt, said, kv), 100, sinks=3, out=out)
+    for r, (a, b) in enumerate(taken):
+        if a == b:
+            continue
+        one = (q[a:b], kc, vc, bt[r:r + 1], torch.tensor([0, b - a], dtype=torch.int32), kv[r:r + 1])
+        ref, weighted = reference(*one, sliding_masks(one, 100, 3))
+        err = ((out[a:b].double().cpu() - ref).abs() <= tolerance(ref, weighted, BF, 600)).all(2).all(1)
+        assert all(bool(err[i - a]) for i in range(a, b) if i not in (2, 9)), (r, err)
+    said = torch.tensor([4, 7, 7, 7, 7, 9], dtype=torch.int32)   # rows 0 .. 3 and 9 .. are nobody's
+    out.fill_(5.0)
+    sliding_attention(*on_gpu(q, kc, vc, bt, said, kv), 100, sinks=3, out=out)
+    assert bool((out[:4] == 5).all()) and bool((out[9:] == 5).all()) and not bool((out[4:9] == 5).any())
+
+
+def test_calls_from_several_threads():
+    from concurrent.futures import ThreadPoolExecutor
+    from monoserve_b200.attention import attention_status, sliding_attention
+    batches = [on_gpu(*make([1, 1 + 20 * s], [3000 + s, 700], 32, 4, 64 * (1 + s % 2), 16, BF, seed=60 + s)) for s in range(4)]
+    want = [sliding_attention(*b, 500, sinks=2) for b in batches]
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        outs = [sliding_attention(*batches[i], 500, sinks=2, stream=stream) for _ in range(20)]
+        stream.synchronize()
+        return all(torch.equal(o, want[i]) for o in outs)
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
+    assert attention_status() == 0
+
+
+@pytest.mark.parametrize("dtype,size", [(FP, 1 << 23), (BF, 1 << 28)])
+@pytest.mark.parametrize("dim,rows", [(64, [1, 30]), (128, [1, 1]), (128, [40, 3])])
+def test_scores_as_large_as_may_be(dtype, size, dim, rows):
+    """Scores of about `size`, exact, most of them a whole step below the largest ones: the output is the mean of those' values.
+    They come in later tiles for some rows, so that references move."""
+    q, kc, vc, bt, start, kv = make(rows, [700, 400], 8, 2, dim, 16, dtype, seed=61)
+    q.zero_(), kc.zero_()
+    q[:, :, 0] = 1 << 8
+    g = torch.Generator().manual_seed(62)
+    kc[..., 0] = torch.randint(-3, 1, kc.shape[:3], generator=g).to(dtype) * (size >> 15) + (size >> 8)   # steps of 2^-7 of `size`
+    batch = (q, kc, vc, bt, start, kv)
+    for window, sinks in ((1 << 30, 0), (200, 3)):
+        check(run_sliding(batch, window, sinks, scale=1.0), batch, sliding_masks(batch, window, sinks), scale=1.0)
